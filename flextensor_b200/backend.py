@@ -161,6 +161,24 @@ def lib():
         handle.ftb_dwconv2d_nchw_f32_multi.restype = i32
         handle.ftb_dwconv2d_nchw_f32_multi.argtypes = ([vp] * 3 + [ctypes.POINTER(vp), i32] + [i64] * 7 + [i32] * 6 +
                                                        [cfgp, vp, vp])
+        size = ctypes.c_size_t
+        f32 = ctypes.c_float
+        signatures = {
+            "ftb_linear": (i32, [i32] + [vp] * 6 + [i64] * 3 + [i32, i32, cfgp, vp, vp]),
+            "ftb_linear_backward_workspace_bytes": (size, [i64] * 3 + [i32]),
+            "ftb_linear_backward": (i32, [i32] + [vp] * 7 + [i64] * 3 + [i32, i32, vp, size, vp, vp]),
+            "ftb_route_experts": (i32, [i32] + [vp] * 4 + [i64] * 3 + [i32] * 4 + [f32, vp]),
+            "ftb_route_experts_backward": (i32, [i32] + [vp] * 4 + [i64] * 3 + [i32, i32, f32, vp]),
+            "ftb_expert_plan": (i32, [vp] * 4 + [i64, i64, vp]),
+            "ftb_expert_linear": (i32, [i32] + [vp] * 7 + [i64] * 5 + [i32] * 3 + [cfgp, vp, vp]),
+            "ftb_expert_linear_backward_workspace_bytes": (size, [i64] * 4 + [i32]),
+            "ftb_expert_linear_backward": (i32, [i32] + [vp] * 9 + [i64] * 5 + [i32] * 3 + [vp, size, vp, vp]),
+            "ftb_expert_combine": (i32, [i32] + [vp] * 5 + [i64] * 3 + [vp]),
+            "ftb_expert_combine_backward": (i32, [i32] + [vp] * 6 + [i64] * 3 + [vp]),
+        }
+        for name, (restype, argtypes) in signatures.items():
+            entry = getattr(handle, name)
+            entry.restype, entry.argtypes = restype, argtypes
         _lib = handle
     return _lib
 
@@ -172,6 +190,9 @@ EXPORTED_SYMBOLS = (
     "ftb_dwconv2d_nchw_f32_multi", "ftb_conv2d_nchw_f32_multi", "ftb_conv2d_pack_filter",
     "ftb_conv2d_nchw_f32_prepacked", "ftb_conv3d_workspace_bytes", "ftb_conv3d_ncdhw_f32",
     "ftb_conv2d_nhwc_f32", "ftb_conv2d_nhwc_workspace_bytes",
+    "ftb_linear", "ftb_linear_backward", "ftb_linear_backward_workspace_bytes", "ftb_route_experts",
+    "ftb_route_experts_backward", "ftb_expert_plan", "ftb_expert_linear", "ftb_expert_linear_backward",
+    "ftb_expert_linear_backward_workspace_bytes", "ftb_expert_combine", "ftb_expert_combine_backward",
 )
 
 
@@ -573,3 +594,313 @@ def dwconv2d_nchw_f32_multi(x, weight, dst_ptrs, bias=None, stride=(1, 1), paddi
             _cfg_ptr(cfg), _status_ptr(status), _stream_ptr(stream))
     if rc:
         raise FtbError(rc, "ftb_dwconv2d_nchw_f32_multi")
+
+
+# ------------------------------------------------------------------ feed-forward operators of language models
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+MAX_EXPERTS, MAX_TOP_K = 1024, 32
+
+
+def _element(t, name):
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("%s must be a bfloat16 or float16 CUDA tensor" % name)
+    return t.dtype
+
+
+def _fits(t, name, shape, dtype, device):
+    """One operand's type, device, layout and shape; its address (None passes through)."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError("%s must be a CUDA tensor" % name)
+    if t.dtype != dtype:
+        raise TypeError("%s must have dtype %s, got %s" % (name, dtype, t.dtype))
+    if t.device != device:
+        raise ValueError("%s is on %s, the call's other tensors on %s" % (name, t.device, device))
+    if t.shape != shape:
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return t.data_ptr()
+
+
+def _one_of(value, table, what):
+    if value not in table:
+        raise ValueError("%s must be one of %s, got %r" % (what, ", ".join(sorted(table)), value))
+    return table[value]
+
+
+def _call(entry, device, stream, *args):
+    """A launcher on ``device``: its current stream unless one is given."""
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    elif stream.device != device:
+        raise ValueError("the stream belongs to %s, the tensors to %s" % (stream.device, device))
+    if torch.cuda.current_device() == device.index:
+        rc = getattr(lib(), entry)(*args, stream.cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib(), entry)(*args, stream.cuda_stream)
+    if rc:
+        raise FtbError(rc, entry)
+
+
+def _status_of(status, device):
+    return None if status is None else _fits(status, "status", (1,), torch.int32, device)
+
+
+def _matrix(t, name, dims):
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError("%s must have %d dimensions" % (name, dims))
+    return t.shape
+
+
+def linear(x, weight, out, bias=None, residual=None, activation="none", gated=False, preact=None, cfg=None, status=None,
+           stream=None):
+    """out[T,N] = act(z) + residual with z = x[T,K] @ weight[N,K].T + bias[N]; ``gated``: weight is [2N,K] (gate rows
+    first), bias [2N], and out = act(z[:, :N]) * z[:, N:] + residual.
+
+    bfloat16 or float16, sums in fp32, one rounding.  ``preact`` ([T,N], gated [T,2N]) receives z for
+    ``linear_backward``.  ``residual`` may be ``out`` itself.  ``activation``: one of ``ACTIVATIONS``.  T may be 0.
+    """
+    dtype = _element(x, "x")
+    act = _one_of(activation, ACTIVATIONS, "activation")
+    tokens, k = _matrix(x, "x", 2)
+    wide = _matrix(weight, "weight", 2)[0]
+    if gated and wide % 2:
+        raise ValueError("a gated weight has an even number of rows, got %d" % wide)
+    n = wide // 2 if gated else wide
+    dev = x.device
+    args = (_fits(x, "x", (tokens, k), dtype, dev), _fits(weight, "weight", (wide, k), dtype, dev),
+            _fits(bias, "bias", (wide,), dtype, dev), _fits(residual, "residual", (tokens, n), dtype, dev),
+            _fits(out, "out", (tokens, n), dtype, dev), _fits(preact, "preact", (tokens, wide), dtype, dev))
+    if args[4] is None:
+        raise TypeError("out must be a CUDA tensor")
+    _call("ftb_linear", dev, stream, DTYPES[dtype], *args, tokens, n, k, act, int(bool(gated)), _cfg_ptr(cfg),
+          _status_of(status, dev))
+
+
+def _workspace_of(workspace, need, device, what):
+    if not isinstance(workspace, torch.Tensor) or not workspace.is_cuda or workspace.device != device:
+        raise ValueError("%s: a workspace of at least %d bytes on %s is required" % (what, need, device))
+    have = workspace.numel() * workspace.element_size()
+    if have < need or not workspace.is_contiguous():
+        raise ValueError("%s: a contiguous workspace of at least %d bytes is required, got %d" % (what, need, have))
+    return workspace.data_ptr(), have
+
+
+def linear_backward_workspace_bytes(tokens, n, k, gated=False):
+    return int(lib().ftb_linear_backward_workspace_bytes(tokens, n, k, int(bool(gated))))
+
+
+def linear_backward(x, weight, dy, dx=None, dweight=None, dbias=None, preact=None, activation="none", gated=False,
+                    workspace=None, status=None, stream=None):
+    """Gradients of ``linear`` from dy[T,N]: dx[T,K], dweight (shape of weight), dbias ([N], gated [2N]); each may be
+    None, not all.  ``preact`` is the z that ``linear`` kept (not read without activation and gate).  The gradient of a
+    residual is dy.  ``workspace``: a CUDA tensor of at least ``linear_backward_workspace_bytes(T, N, K, gated)`` bytes,
+    not shared with a call that may run at the same time.  T may be 0: dweight and dbias are then zeros.
+    """
+    dtype = _element(x, "x")
+    act = _one_of(activation, ACTIVATIONS, "activation")
+    tokens, k = _matrix(x, "x", 2)
+    wide = _matrix(weight, "weight", 2)[0]
+    if gated and wide % 2:
+        raise ValueError("a gated weight has an even number of rows, got %d" % wide)
+    n = wide // 2 if gated else wide
+    dev = x.device
+    if (gated or act) and preact is None:
+        raise ValueError("preact (the z of the forward call) is needed for the derivative of the activation")
+    if dx is None and dweight is None and dbias is None:
+        raise ValueError("at least one of dx, dweight and dbias")
+    args = (_fits(x, "x", (tokens, k), dtype, dev), _fits(weight, "weight", (wide, k), dtype, dev),
+            _fits(dy, "dy", (tokens, n), dtype, dev), _fits(preact, "preact", (tokens, wide), dtype, dev),
+            _fits(dx, "dx", (tokens, k), dtype, dev), _fits(dweight, "dweight", (wide, k), dtype, dev),
+            _fits(dbias, "dbias", (wide,), dtype, dev))
+    if args[2] is None:
+        raise TypeError("dy must be a CUDA tensor")
+    need = linear_backward_workspace_bytes(tokens, n, k, gated)
+    ws = _workspace_of(workspace, need, dev, "linear_backward")
+    _call("ftb_linear_backward", dev, stream, DTYPES[dtype], *args, tokens, n, k, act, int(bool(gated)), *ws,
+          _status_of(status, dev))
+
+
+def route_experts(logits, ids, weights, bias=None, scoring="softmax", groups=1, top_groups=1, renormalize=True, scale=1.0,
+                  stream=None):
+    """The top_k experts of every token: ids[T,top_k] (int32, best first, equal scores in the order of their index) and
+    weights[T,top_k] (float32) from logits[T,E] (float32, bfloat16 or float16).
+
+    Scores are the softmax or sigmoid of the logits; ``bias`` (float32 [E]) takes part in the choice, not in the
+    weights.  With ``groups`` > 1 the experts are that many equal runs, valued by the sum of their two best scores, and
+    only the ``top_groups`` best runs stay.  ``renormalize``: weights are divided by their sum; then times ``scale``.
+    A logit of -inf or NaN has score 0.  At most 1024 experts, top_k 32, 32 groups.
+    """
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in DTYPES:
+        raise TypeError("logits must be a float32, bfloat16 or float16 CUDA tensor")
+    kind = _one_of(scoring, SCORINGS, "scoring")
+    tokens, experts = _matrix(logits, "logits", 2)
+    top_k = _matrix(ids, "ids", 2)[1]
+    dev = logits.device
+    if not 1 <= top_groups <= groups or experts % groups:
+        raise ValueError("%d experts do not split into %d groups of which %d stay" % (experts, groups, top_groups))
+    if not 1 <= top_k <= experts // groups * top_groups:
+        raise ValueError("top_k %d of %d experts" % (top_k, experts // groups * top_groups))
+    args = (_fits(logits, "logits", (tokens, experts), logits.dtype, dev),
+            _fits(bias, "bias", (experts,), torch.float32, dev), _fits(ids, "ids", (tokens, top_k), torch.int32, dev),
+            _fits(weights, "weights", (tokens, top_k), torch.float32, dev))
+    if args[3] is None:
+        raise TypeError("weights must be a CUDA tensor")
+    _call("ftb_route_experts", dev, stream, DTYPES[logits.dtype], *args, tokens, experts, top_k, kind, groups, top_groups,
+          int(bool(renormalize)), float(scale))
+
+
+def route_experts_backward(logits, ids, dweights, dlogits, scoring="softmax", renormalize=True, scale=1.0, stream=None):
+    """dlogits[T,E] (type of the logits) from dweights[T,top_k] (float32) of ``route_experts`` with the same settings;
+    the choice itself has no gradient.  An id outside [0, E) adds nothing."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in DTYPES:
+        raise TypeError("logits must be a float32, bfloat16 or float16 CUDA tensor")
+    kind = _one_of(scoring, SCORINGS, "scoring")
+    tokens, experts = _matrix(logits, "logits", 2)
+    top_k = _matrix(ids, "ids", 2)[1]
+    dev = logits.device
+    args = (_fits(logits, "logits", (tokens, experts), logits.dtype, dev),
+            _fits(ids, "ids", (tokens, top_k), torch.int32, dev),
+            _fits(dweights, "dweights", (tokens, top_k), torch.float32, dev),
+            _fits(dlogits, "dlogits", (tokens, experts), logits.dtype, dev))
+    if args[2] is None or args[3] is None:
+        raise TypeError("dweights and dlogits must be CUDA tensors")
+    _call("ftb_route_experts_backward", dev, stream, DTYPES[logits.dtype], *args, tokens, experts, top_k, kind,
+          int(bool(renormalize)), float(scale))
+
+
+class ExpertPlan(object):
+    """Where the rows of ``tokens`` x ``top_k`` expert ids lie when they are sorted by expert; ``expert_plan`` fills it.
+
+    offsets [experts + 1]  first place of each expert; the last entry is the number of rows that have one
+    order   [rows]         place -> row (token * top_k + slot); -1 past the last place
+    slots   [rows]         row -> place; -1 where the row's id is outside [0, experts)
+    """
+
+    def __init__(self, tokens, top_k, experts, device="cuda"):
+        if tokens < 0 or not 1 <= top_k <= MAX_TOP_K or not 1 <= experts <= MAX_EXPERTS:
+            raise ValueError("a plan needs tokens >= 0, top_k in 1..%d and experts in 1..%d" % (MAX_TOP_K, MAX_EXPERTS))
+        self.tokens, self.top_k, self.experts = int(tokens), int(top_k), int(experts)
+        self.rows = self.tokens * self.top_k
+        self.offsets = torch.zeros(self.experts + 1, dtype=torch.int32, device=device)
+        self.order = torch.full((self.rows,), -1, dtype=torch.int32, device=device)
+        self.slots = torch.full((self.rows,), -1, dtype=torch.int32, device=device)
+        self.device = self.offsets.device
+
+
+def _plan_of(plan):
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError("plan must be an ExpertPlan")
+    return plan
+
+
+def expert_plan(ids, plan, stream=None):
+    """Fills ``plan`` from ids[tokens, top_k] (int32): a stable sort of the rows by expert, ids outside [0, experts)
+    dropped."""
+    _plan_of(plan)
+    at = _fits(ids, "ids", (plan.tokens, plan.top_k), torch.int32, plan.device)
+    if at is None:
+        raise TypeError("ids must be a CUDA tensor")
+    _call("ftb_expert_plan", plan.device, stream, at, plan.offsets.data_ptr(), plan.order.data_ptr(),
+          plan.slots.data_ptr(), plan.rows, plan.experts)
+
+
+def expert_linear(x, weight, plan, out, bias=None, activation="none", gated=False, gather=False, preact=None, cfg=None,
+                  status=None, stream=None):
+    """For every place p of expert e in ``plan``: out[p] = act(x-row @ weight[e].T + bias[e]), gated as in ``linear``.
+
+    weight [E,N,K] (gated [E,2N,K]), bias [E,N] ([E,2N]), out [rows,N], preact [rows,N] ([rows,2N]).  ``gather``: x is
+    [tokens,K] and place p reads its token's row; otherwise x is [rows,K], sorted.  Places past the last row
+    (``plan.offsets[-1]``) are left as they were.
+    """
+    dtype = _element(x, "x")
+    act = _one_of(activation, ACTIVATIONS, "activation")
+    _plan_of(plan)
+    k = _matrix(x, "x", 2)[1]
+    wide = _matrix(weight, "weight", 3)[1]
+    if gated and wide % 2:
+        raise ValueError("a gated weight has an even number of rows, got %d" % wide)
+    n = wide // 2 if gated else wide
+    dev, rows, experts = plan.device, plan.rows, plan.experts
+    args = (_fits(x, "x", (plan.tokens if gather else rows, k), dtype, dev),
+            _fits(weight, "weight", (experts, wide, k), dtype, dev), _fits(bias, "bias", (experts, wide), dtype, dev),
+            plan.offsets.data_ptr(), plan.order.data_ptr(), _fits(out, "out", (rows, n), dtype, dev),
+            _fits(preact, "preact", (rows, wide), dtype, dev))
+    if args[5] is None:
+        raise TypeError("out must be a CUDA tensor")
+    _call("ftb_expert_linear", dev, stream, DTYPES[dtype], *args, rows, plan.top_k, experts, n, k, act, int(bool(gated)),
+          int(bool(gather)), _cfg_ptr(cfg), _status_of(status, dev))
+
+
+def expert_linear_backward_workspace_bytes(plan, n, k, gated=False):
+    return int(lib().ftb_expert_linear_backward_workspace_bytes(_plan_of(plan).rows, plan.experts, n, k, int(bool(gated))))
+
+
+def expert_linear_backward(x, weight, plan, dy, dx=None, dweight=None, dbias=None, preact=None, activation="none",
+                           gated=False, gather=False, workspace=None, status=None, stream=None):
+    """Gradients of ``expert_linear`` from dy[rows,N]: dx[rows,K] by place, dweight (shape of weight), dbias (shape of
+    bias), zeros for an expert without rows; each may be None, not all.  With ``gather`` the gradient of x is the sum of
+    its places: ``expert_combine(dx, plan, out)``.  Places past the last row are neither read nor written.
+    ``workspace``: at least ``expert_linear_backward_workspace_bytes(plan, N, K, gated)`` bytes."""
+    dtype = _element(x, "x")
+    act = _one_of(activation, ACTIVATIONS, "activation")
+    _plan_of(plan)
+    k = _matrix(x, "x", 2)[1]
+    wide = _matrix(weight, "weight", 3)[1]
+    if gated and wide % 2:
+        raise ValueError("a gated weight has an even number of rows, got %d" % wide)
+    n = wide // 2 if gated else wide
+    if (gated or act) and preact is None:
+        raise ValueError("preact (the z of the forward call) is needed for the derivative of the activation")
+    if dx is None and dweight is None and dbias is None:
+        raise ValueError("at least one of dx, dweight and dbias")
+    dev, rows, experts = plan.device, plan.rows, plan.experts
+    args = (_fits(x, "x", (plan.tokens if gather else rows, k), dtype, dev),
+            _fits(weight, "weight", (experts, wide, k), dtype, dev), plan.offsets.data_ptr(), plan.order.data_ptr(),
+            _fits(dy, "dy", (rows, n), dtype, dev), _fits(preact, "preact", (rows, wide), dtype, dev),
+            _fits(dx, "dx", (rows, k), dtype, dev), _fits(dweight, "dweight", (experts, wide, k), dtype, dev),
+            _fits(dbias, "dbias", (experts, wide), dtype, dev))
+    if args[4] is None:
+        raise TypeError("dy must be a CUDA tensor")
+    need = expert_linear_backward_workspace_bytes(plan, n, k, gated)
+    ws = _workspace_of(workspace, need, dev, "expert_linear_backward")
+    _call("ftb_expert_linear_backward", dev, stream, DTYPES[dtype], *args, rows, plan.top_k, experts, n, k, act,
+          int(bool(gated)), int(bool(gather)), *ws, _status_of(status, dev))
+
+
+def expert_combine(y, plan, out, weights=None, residual=None, stream=None):
+    """out[T,N] = residual + sum over a token's slots j of weights[T,top_k][., j] (float32, ones if None) times its row of
+    y[rows,N]; dropped rows add nothing.  ``residual`` may be ``out`` itself."""
+    dtype = _element(y, "y")
+    _plan_of(plan)
+    n = _matrix(y, "y", 2)[1]
+    dev = plan.device
+    args = (_fits(y, "y", (plan.rows, n), dtype, dev), plan.slots.data_ptr(),
+            _fits(weights, "weights", (plan.tokens, plan.top_k), torch.float32, dev),
+            _fits(residual, "residual", (plan.tokens, n), dtype, dev), _fits(out, "out", (plan.tokens, n), dtype, dev))
+    if args[4] is None:
+        raise TypeError("out must be a CUDA tensor")
+    _call("ftb_expert_combine", dev, stream, DTYPES[dtype], *args, plan.tokens, plan.top_k, n)
+
+
+def expert_combine_backward(dout, plan, y=None, weights=None, dy=None, dweights=None, stream=None):
+    """Gradients of ``expert_combine`` from dout[T,N]: dy[rows,N] by place, dweights[T,top_k] (float32, needs y; 0 for a
+    dropped row); either may be None.  The gradient of the residual is dout."""
+    dtype = _element(dout, "dout")
+    _plan_of(plan)
+    n = _matrix(dout, "dout", 2)[1]
+    if dy is None and dweights is None:
+        raise ValueError("at least one of dy and dweights")
+    if dweights is not None and y is None:
+        raise ValueError("dweights needs y")
+    dev = plan.device
+    args = (_fits(dout, "dout", (plan.tokens, n), dtype, dev), _fits(y, "y", (plan.rows, n), dtype, dev),
+            plan.slots.data_ptr(), _fits(weights, "weights", (plan.tokens, plan.top_k), torch.float32, dev),
+            _fits(dy, "dy", (plan.rows, n), dtype, dev),
+            _fits(dweights, "dweights", (plan.tokens, plan.top_k), torch.float32, dev))
+    _call("ftb_expert_combine_backward", dev, stream, DTYPES[dtype], *args, plan.tokens, plan.top_k, n)

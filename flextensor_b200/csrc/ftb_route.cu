@@ -1,0 +1,481 @@
+// Routing of tokens to experts and its gradient: one warp per token, the token's logits in registers (a lane holds VPL
+// neighbouring experts).  Forward and backward read every logit once; bytes bound long batches, launch latency short
+// ones.
+//
+// The choice is defined on exact scores, so that neither the type nor the rounding of a softmax decides between two
+// experts.  Without bias and groups both scorings are monotone and the logits themselves are compared.  Otherwise
+// scores are computed in fp32 with a bound on their error; where two values that decide the result lie closer than
+// that bound, the warp computes the row's scores again in 64 bits and chooses by those.
+#include "ftb_lm.cuh"
+
+namespace ftb {
+
+constexpr int kMaxGroups = 32;  // a lane holds a group's value
+constexpr unsigned kAll = 0xffffffffu;
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;
+  int* ids;
+  float* weights;
+  const float* dweights;
+  void* dlogits;
+  long long tokens;
+  int experts, top_k, scoring, groups, top_groups, renorm, vec;
+  float scale;
+};
+
+template <typename T>
+__device__ __forceinline__ float load_logit(const T* p);
+template <>
+__device__ __forceinline__ float load_logit<float>(const float* p) { return *p; }
+template <>
+__device__ __forceinline__ float load_logit<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+template <>
+__device__ __forceinline__ float load_logit<__half>(const __half* p) { return __half2float(*p); }
+
+__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_logit(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_logit(__half* p, float v) { *p = __float2half_rn(v); }
+
+// NaN counts as -inf; -0 becomes 0, which orders equal to it.
+__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+
+// The lane's VPL logits; -inf past the last expert.
+template <typename T, int VPL>
+__device__ __forceinline__ void load_row(const T* row, int experts, int lane, bool vec, float (&x)[VPL]) {
+  const int e0 = lane * VPL;
+  constexpr int PER = 16 / static_cast<int>(sizeof(T));
+  if constexpr (VPL % PER == 0) {
+    if (vec && e0 + VPL <= experts) {
+#pragma unroll
+      for (int q = 0; q < VPL / PER; ++q) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(row + e0 + q * PER);
+        const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[q * PER + i] = clean(load_logit<T>(t + i));
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) x[v] = e0 + v < experts ? clean(load_logit<T>(row + e0 + v)) : -INFINITY;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
+  return v;
+}
+template <typename S>
+__device__ __forceinline__ S warp_sum(S v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
+  return v;
+}
+
+// Whole numbers in the order of the floating values (never 0, which stands for "none left").
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t order_key(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  return b ^ ((b >> 63) ? ~0ull : (1ull << 63));
+}
+__device__ __forceinline__ double key_value(uint64_t k) {
+  return __longlong_as_double(static_cast<long long>(k ^ ((k >> 63) ? (1ull << 63) : ~0ull)));
+}
+__device__ __forceinline__ uint32_t key_max(uint32_t k) { return __reduce_max_sync(kAll, k); }
+__device__ __forceinline__ uint64_t key_max(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(kAll, static_cast<uint32_t>(k >> 32));
+  const uint32_t lo = __reduce_max_sync(kAll, (k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+// The `count` largest of the available values c, best first, ties to the lowest index: lane j gets the index of the
+// j-th.  `near` is set when two neighbours in that order, the last chosen and the first left out among them, are at
+// most `tol` apart.
+template <typename S, int VPL>
+__device__ __forceinline__ int pick(const S (&c)[VPL], uint32_t avail, int count, S tol, int lane, bool* near) {
+  int mine = 0;
+  S prev = S(0);
+  for (int j = 0; j <= count; ++j) {
+    S best = S(0);
+    int at = -1;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (((avail >> v) & 1u) && (at < 0 || c[v] > best)) {
+        best = c[v];
+        at = v;
+      }
+    decltype(order_key(best)) key = 0;
+    if (at >= 0) key = order_key(best);
+    const auto top = key_max(key);
+    if (top == 0) break;  // none left
+    const S cur = key_value(top);
+    if (j > 0 && prev - cur <= tol) *near = true;
+    prev = cur;
+    if (j == count) break;
+    const int winner = __ffs(__ballot_sync(kAll, key == top)) - 1;
+    const int id = __shfl_sync(kAll, lane * VPL + at, winner);
+    if (lane == winner) avail &= ~(1u << at);
+    if (lane == j) mine = id;
+  }
+  return mine;
+}
+
+template <typename S>
+__device__ __forceinline__ void merge_top2(S& a, S& b, S oa, S ob) {
+  // the two largest of two ordered pairs
+  const S lo = a > oa ? oa : a;
+  a = a > oa ? a : oa;
+  b = b > ob ? b : ob;
+  b = b > lo ? b : lo;
+}
+
+// Bits of the lane's values that lie in the kept groups.
+template <typename S, int VPL>
+__device__ __forceinline__ uint32_t keep_groups(const RouteArgs& p, const S (&c)[VPL], uint32_t avail, S tol, int lane,
+                                                bool* near) {
+  const int size = p.experts / p.groups, e0 = lane * VPL;
+  const S none = static_cast<S>(-INFINITY);
+  S value = none;  // of group `lane`
+  const int lanes = size / VPL;
+  if (size % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+    // a lane's values share a group, a group is a run of 2^n lanes
+    S a = none, b = none;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if ((avail >> v) & 1u) merge_top2(a, b, c[v], none);
+    for (int d = 1; d < lanes; d <<= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
+    const S sum = size > 1 ? a + b : a;
+    value = __shfl_sync(kAll, sum, lane < p.groups ? lane * lanes : 0);
+  } else {
+    for (int g = 0; g < p.groups; ++g) {
+      S a = none, b = none;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v)
+        if (((avail >> v) & 1u) && (e0 + v) / size == g) merge_top2(a, b, c[v], none);
+#pragma unroll
+      for (int d = 16; d; d >>= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
+      if (lane == g) value = size > 1 ? a + b : a;
+    }
+  }
+  if (value != value) value = none;
+  const S one[1] = {value};
+  const int mine = pick<S, 1>(one, lane < p.groups ? 1u : 0u, p.top_groups, 2 * tol, lane, near);
+  uint32_t kept = __reduce_or_sync(kAll, lane < p.top_groups ? 1u << mine : 0u);
+  uint32_t left = 0;
+#pragma unroll
+  for (int v = 0; v < VPL; ++v)
+    if (((avail >> v) & 1u) && ((kept >> ((e0 + v) / size)) & 1u)) left |= 1u << v;
+  return left;
+}
+
+// exp(x - m) with the limits that a row of infinities has: the largest share the mass, a row of -inf has none.
+__device__ __forceinline__ float exp_below(float x, float m) { return m == -INFINITY ? 0.0f : x == m ? 1.0f : expf(x - m); }
+
+template <int VPL>
+__device__ __noinline__ int choose_exactly(const RouteArgs& p, const float (&x)[VPL], uint32_t avail, float m, int lane) {
+  double c[VPL];
+  double sum = 0.0;
+  const int e0 = lane * VPL;
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) {
+    const double d = static_cast<double>(x[v]);
+    if (p.scoring == FTB_SCORE_SIGMOID) c[v] = 1.0 / (1.0 + exp(-d));
+    else c[v] = m == -INFINITY ? 0.0 : x[v] == m ? 1.0 : exp(d - static_cast<double>(m));
+    sum += ((avail >> v) & 1u) ? c[v] : 0.0;
+  }
+  sum = warp_sum(sum);
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) {
+    if (p.scoring == FTB_SCORE_SOFTMAX) c[v] = sum > 0.0 ? c[v] / sum : 0.0;
+    if (p.bias && ((avail >> v) & 1u)) c[v] += static_cast<double>(p.bias[e0 + v]);
+    c[v] = c[v] != c[v] ? -INFINITY : c[v] + 0.0;
+  }
+  bool near = false;
+  if (p.groups > 1) avail = keep_groups<double, VPL>(p, c, avail, -1.0, lane, &near);
+  return pick<double, VPL>(c, avail, p.top_k, -1.0, lane, &near);
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
+  const int lane = threadIdx.x & 31;
+  const long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (t >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + t * p.experts;
+  const int e0 = lane * VPL;
+  float x[VPL];
+  load_row<T, VPL>(row, p.experts, lane, p.vec != 0, x);
+  const int have = min(max(p.experts - e0, 0), VPL);
+  const uint32_t avail = have >= 32 ? kAll : (1u << have) - 1u;
+
+  const bool sigmoid = p.scoring == FTB_SCORE_SIGMOID;
+  const bool by_logit = !p.bias && p.groups == 1;
+  float m = -INFINITY, total = 0.0f;
+  const bool need_sum = !sigmoid && (!by_logit || !p.renorm);
+  if (!sigmoid) {
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) m = fmaxf(m, x[v]);
+    m = warp_max(m);
+  }
+  int mine;
+  if (by_logit) {
+    bool near = false;
+    mine = pick<float, VPL>(x, avail, p.top_k, -1.0f, lane, &near);
+    if (need_sum) {
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) total += exp_below(x[v], m);
+      total = warp_sum(total);
+    }
+  } else {
+    float c[VPL];
+    float most = 0.0f;  // largest magnitude that enters a sum: what the error bound scales with
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      c[v] = sigmoid ? 1.0f / (1.0f + expf(-x[v])) : exp_below(x[v], m);
+      total += ((avail >> v) & 1u) ? c[v] : 0.0f;
+    }
+    total = warp_sum(total);
+    const float inv = sigmoid ? 1.0f : total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      c[v] *= inv;
+      most = fmaxf(most, ((avail >> v) & 1u) ? c[v] : 0.0f);
+      if (p.bias && ((avail >> v) & 1u)) {
+        const float b = p.bias[e0 + v];
+        c[v] += b;
+        if (fabsf(b) < INFINITY) most = fmaxf(most, fabsf(b));
+      }
+      c[v] = clean(c[v]);
+    }
+    // exp and the reciprocals are good to a few units of 2^-24, the sum over the row to about 8 more
+    const float tol = 2e-6f * warp_max(most);
+    bool near = false;
+    uint32_t left = avail;
+    if (p.groups > 1) left = keep_groups<float, VPL>(p, c, avail, tol, lane, &near);
+    mine = pick<float, VPL>(c, left, p.top_k, tol, lane, &near);
+    if (near) mine = choose_exactly<VPL>(p, x, avail, m, lane);
+  }
+
+  // weights: lane j < top_k has the j-th expert
+  const bool active = lane < p.top_k;
+  const float l = active ? clean(load_logit<T>(row + mine)) : -INFINITY;
+  float w;
+  if (sigmoid) {
+    w = active ? 1.0f / (1.0f + expf(-l)) : 0.0f;
+    if (p.renorm) {
+      float s = warp_sum(w);
+      if (s < 1e-30f) {
+        // every chosen score underflows or nearly so: the ratios of exp(l), which 1 / (1 + exp(-l)) tends to
+        const float top = warp_max(l);
+        w = active ? exp_below(l, top) : 0.0f;
+        s = warp_sum(w);
+      }
+      w = s > 0.0f ? w / s : 0.0f;
+    }
+  } else if (p.renorm) {
+    const float top = warp_max(l);
+    w = active ? exp_below(l, top) : 0.0f;
+    const float s = warp_sum(w);
+    w = s > 0.0f ? w / s : 0.0f;
+  } else {
+    w = total > 0.0f ? exp_below(l, m) / total : 0.0f;
+  }
+  if (active) {
+    p.ids[t * p.top_k + lane] = mine;
+    p.weights[t * p.top_k + lane] = w * p.scale;
+  }
+}
+
+// d logits.  With the chosen scores scaled to one (r = s / sum of s), both scorings give
+//   ds r-part: g_j = scale * (dw_j - sum_i r_i dw_i);   softmax: dl_j = r_j g_j;   sigmoid: dl_j = r_j g_j (1 - s_j);
+// without scaling softmax gives dl_e = s_e (g_e - sum_j g_j s_j) for every expert and sigmoid dl_j = g_j s_j (1 - s_j).
+// An expert that a row names twice gets both parts, added in the order of the slots.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) {
+  __shared__ float grad[8][32 * VPL];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long t = static_cast<long long>(blockIdx.x) * 8 + warp;
+  if (t >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + t * p.experts;
+  T* drow = static_cast<T*>(p.dlogits) + t * p.experts;
+  const int e0 = lane * VPL;
+  const bool sigmoid = p.scoring == FTB_SCORE_SIGMOID;
+  int id = lane < p.top_k ? p.ids[t * p.top_k + lane] : -1;
+  const bool active = id >= 0 && id < p.experts;
+  if (!active) id = 0;
+  const float dw = active ? p.dweights[t * p.top_k + lane] * p.scale : 0.0f;
+  const float l = active ? clean(load_logit<T>(row + id)) : -INFINITY;
+  const bool full = !sigmoid && !p.renorm;  // every logit has a gradient
+  float x[VPL];
+  float m = -INFINITY, total = 0.0f;
+  if (full) {
+    load_row<T, VPL>(row, p.experts, lane, p.vec != 0, x);
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) m = fmaxf(m, x[v]);
+    m = warp_max(m);
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      x[v] = exp_below(x[v], m);
+      total += x[v];
+    }
+    total = warp_sum(total);
+  }
+  float part;  // what the lane's slot adds to its expert's gradient (full: its g)
+  float back = 0.0f;
+  if (full) {
+    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) x[v] *= inv;
+    part = dw;
+    back = warp_sum(active ? dw * exp_below(l, m) * inv : 0.0f);
+  } else {
+    const float s = sigmoid ? (active ? 1.0f / (1.0f + expf(-l)) : 0.0f) : 0.0f;
+    if (p.renorm) {
+      float r = s, sum = sigmoid ? warp_sum(s) : 0.0f;
+      if (!sigmoid || sum < 1e-30f) {
+        const float top = warp_max(l);
+        r = active ? exp_below(l, top) : 0.0f;
+        sum = warp_sum(r);
+      }
+      r = sum > 0.0f ? r / sum : 0.0f;
+      const float mean = warp_sum(r * dw);
+      part = active ? r * (dw - mean) : 0.0f;
+    } else {
+      part = s * dw;
+    }
+    // 1 - s without cancellation
+    if (sigmoid) part = active ? part * (1.0f / (1.0f + expf(l))) : 0.0f;
+  }
+  float* mine = grad[warp];
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) mine[v * 32 + lane] = 0.0f;
+  __syncwarp();
+  for (int j = 0; j < p.top_k; ++j) {
+    if (lane == j && active) mine[id] += part;
+    __syncwarp();
+  }
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) x[v] = full ? x[v] * (mine[e0 + v] - back) : mine[e0 + v];
+  constexpr int PER = 16 / static_cast<int>(sizeof(T));
+  if constexpr (VPL % PER == 0) {
+    if (p.vec && e0 + VPL <= p.experts) {
+#pragma unroll
+      for (int q = 0; q < VPL / PER; ++q) {
+        uint4 raw;
+        T* o = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) store_logit(o + i, x[q * PER + i]);
+        *reinterpret_cast<uint4*>(drow + e0 + q * PER) = raw;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VPL; ++v)
+    if (e0 + v < p.experts) store_logit(drow + e0 + v, x[v]);
+}
+
+template <typename T, int VPL>
+static void launch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
+  const unsigned blocks = static_cast<unsigned>((p.tokens + 7) / 8);
+  if (backward) route_backward_kernel<T, VPL><<<blocks, 256, 0, stream>>>(p);
+  else route_kernel<T, VPL><<<blocks, 256, 0, stream>>>(p);
+}
+
+template <typename T>
+static void dispatch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
+  const int per = (p.experts + 31) / 32;
+  if (per <= 1) launch_route<T, 1>(p, backward, stream);
+  else if (per <= 2) launch_route<T, 2>(p, backward, stream);
+  else if (per <= 4) launch_route<T, 4>(p, backward, stream);
+  else if (per <= 8) launch_route<T, 8>(p, backward, stream);
+  else if (per <= 16) launch_route<T, 16>(p, backward, stream);
+  else launch_route<T, 32>(p, backward, stream);
+}
+
+static int route_checks(int dtype, int64_t tokens, int64_t experts, int64_t top_k, int scoring) {
+  if (dtype < FTB_F32 || dtype > FTB_F16) return FTB_E_BAD_ARG;
+  if (tokens < 0 || experts <= 0 || top_k <= 0) return FTB_E_BAD_ARG;
+  if (scoring != FTB_SCORE_SOFTMAX && scoring != FTB_SCORE_SIGMOID) return FTB_E_BAD_ARG;
+  if (experts > FTB_MAX_EXPERTS || top_k > FTB_MAX_TOP_K || tokens > (1ll << 30)) return FTB_E_TOO_LARGE;
+  return FTB_OK;
+}
+
+static int run_route(int dtype, RouteArgs& p, bool backward, cudaStream_t stream) {
+  const int rc = device_ok();
+  if (rc) return rc;
+  const int esize = dtype == FTB_F32 ? 4 : 2;
+  p.vec = (p.experts * esize) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 &&
+          (!backward || (reinterpret_cast<uintptr_t>(p.dlogits) & 15) == 0);
+  if (dtype == FTB_F32) dispatch_route<float>(p, backward, stream);
+  else if (dtype == FTB_BF16) dispatch_route<__nv_bfloat16>(p, backward, stream);
+  else dispatch_route<__half>(p, backward, stream);
+  count_launch();
+  return launch_status(cudaSuccess);
+}
+
+}  // namespace ftb
+
+extern "C" {
+
+int ftb_route_experts(int dtype, const void* logits, const float* bias, int32_t* ids, float* weights, int64_t tokens,
+                      int64_t experts, int64_t top_k, int scoring, int groups, int top_groups, int renormalize,
+                      float scale, void* stream) {
+  using namespace ftb;
+  const int rc = route_checks(dtype, tokens, experts, top_k, scoring);
+  if (rc) return rc;
+  if (groups < 1 || top_groups < 1 || top_groups > groups || experts % groups != 0) return FTB_E_BAD_ARG;
+  if (groups > kMaxGroups) return FTB_E_TOO_LARGE;
+  if (top_k > experts / groups * top_groups) return FTB_E_BAD_ARG;
+  if (tokens == 0) return FTB_OK;
+  if (!logits || !ids || !weights) return FTB_E_BAD_ARG;
+  RouteArgs p;
+  memset(&p, 0, sizeof(p));
+  p.logits = logits;
+  p.bias = bias;
+  p.ids = ids;
+  p.weights = weights;
+  p.tokens = tokens;
+  p.experts = static_cast<int>(experts);
+  p.top_k = static_cast<int>(top_k);
+  p.scoring = scoring;
+  p.groups = groups;
+  p.top_groups = top_groups;
+  p.renorm = renormalize != 0;
+  p.scale = scale;
+  return run_route(dtype, p, false, static_cast<cudaStream_t>(stream));
+}
+
+int ftb_route_experts_backward(int dtype, const void* logits, const int32_t* ids, const float* dweights, void* dlogits,
+                               int64_t tokens, int64_t experts, int64_t top_k, int scoring, int renormalize, float scale,
+                               void* stream) {
+  using namespace ftb;
+  const int rc = route_checks(dtype, tokens, experts, top_k, scoring);
+  if (rc) return rc;
+  if (tokens == 0) return FTB_OK;
+  if (!logits || !ids || !dweights || !dlogits) return FTB_E_BAD_ARG;
+  RouteArgs p;
+  memset(&p, 0, sizeof(p));
+  p.logits = logits;
+  p.ids = const_cast<int32_t*>(ids);
+  p.dweights = dweights;
+  p.dlogits = dlogits;
+  p.tokens = tokens;
+  p.experts = static_cast<int>(experts);
+  p.top_k = static_cast<int>(top_k);
+  p.scoring = scoring;
+  p.groups = 1;
+  p.top_groups = 1;
+  p.renorm = renormalize != 0;
+  p.scale = scale;
+  return run_route(dtype, p, true, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

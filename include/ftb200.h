@@ -258,6 +258,82 @@ int ftb_dwconv2d_nchw_f32_multi(const float* in, const float* weight, const floa
                                 int64_t r, int64_t s, int stride_h, int stride_w, int pad_h, int pad_w,
                                 int dil_h, int dil_w, const ftb_config* cfg, int* status, void* stream);
 
+/* ---------------------------------------------------------------- feed-forward operators of language models
+ * No counterpart in the reference, whose contractions end with the plain product (flextensor/nn/ops.py:1074-1158).
+ * Conventions beyond the ones above: tensors are contiguous; `tokens` or `rows` of 0 is a call with nothing to
+ * multiply (gradients of weights and biases are then written as zeros); matrix elements are 16 bits wide, every sum is
+ * carried in fp32 and rounded once when it is stored.  Row pitches and bases that are multiples of 16 bytes (`k`, and
+ * for gradients nothing else, a multiple of 8) run on tcgen05; other sizes run on a CUDA-core kernel of the library. */
+enum ftb_dtype { FTB_F32 = 0, FTB_BF16 = 1, FTB_F16 = 2 };
+enum ftb_activation { FTB_ACT_NONE = 0, FTB_ACT_RELU = 1, FTB_ACT_GELU = 2 /* erf */, FTB_ACT_GELU_TANH = 3, FTB_ACT_SILU = 4 };
+enum ftb_scoring { FTB_SCORE_SOFTMAX = 0, FTB_SCORE_SIGMOID = 1 };
+#define FTB_MAX_EXPERTS 1024
+#define FTB_MAX_TOP_K 32
+
+/* out[tokens,n] = act(z) + residual with z = x[tokens,k] . w[n,k]^T + bias[n]; gated: w is [2n,k] (gate rows, then the
+ * others), bias [2n], out = act(z[:, :n]) * z[:, n:] + residual.  `preact` (may be null) receives z ([tokens, n or 2n])
+ * for the backward pass.  bias and residual may be null; all tensors have `dtype` (FTB_BF16 or FTB_F16).  residual may
+ * be `out` itself.  Knobs of `cfg`: tile_n (tokens per tile: 16, 32, 64, 128, or 256 with cluster 2), cluster (2: tile_n 128 or 256), stages,
+ * split_k (1, 2, 4 or 8 CTAs of a cluster share a tile's reduction; cluster 1, tile_n <= 64). */
+int ftb_linear(int dtype, const void* x, const void* w, const void* bias, const void* residual, void* out, void* preact,
+               int64_t tokens, int64_t n, int64_t k, int activation, int gated, const ftb_config* cfg, int* status,
+               void* stream);
+
+/* Gradients of ftb_linear from dy[tokens,n] and the saved z: dz = dy * act'(z) (gated: both halves), dx = dz . w,
+ * dw = dz^T . x, db = sum of dz over the tokens.  dx, dw, db may each be null; preact may be null when the activation
+ * is none and there is no gate.  The gradient of the residual is dy.  dz is held in `dtype` in the workspace (16-byte
+ * aligned, ftb_linear_backward_workspace_bytes); db is summed from fp32 values in a fixed order. */
+size_t ftb_linear_backward_workspace_bytes(int64_t tokens, int64_t n, int64_t k, int gated);
+int ftb_linear_backward(int dtype, const void* x, const void* w, const void* dy, const void* preact, void* dx, void* dw,
+                        void* db, int64_t tokens, int64_t n, int64_t k, int activation, int gated, void* workspace,
+                        size_t workspace_bytes, int* status, void* stream);
+
+/* Experts of each token: scores s = softmax or sigmoid of logits[tokens,experts] (FTB_F32, FTB_BF16 or FTB_F16); choice
+ * c = s + bias[experts] (bias may be null).  With groups > 1 the experts are `groups` equal runs, a group's value is the
+ * sum of its two largest c, and only the `top_groups` best groups stay.  ids[tokens,top_k] are the experts of largest c,
+ * best first, equal values in the order of their index; the order is that of exact scores (near ties are resolved in 64
+ * bits).  weights[tokens,top_k] = s of the chosen (without the bias), divided by their sum if `renormalize`, times scale.
+ * A logit that is -inf or NaN counts as a score of zero; a row without any other has weights of zero. */
+int ftb_route_experts(int dtype, const void* logits, const float* bias, int32_t* ids, float* weights, int64_t tokens,
+                      int64_t experts, int64_t top_k, int scoring, int groups, int top_groups, int renormalize,
+                      float scale, void* stream);
+/* dlogits[tokens,experts] (type of the logits) from dweights[tokens,top_k]; ids outside [0, experts) have no gradient. */
+int ftb_route_experts_backward(int dtype, const void* logits, const int32_t* ids, const float* dweights, void* dlogits,
+                               int64_t tokens, int64_t experts, int64_t top_k, int scoring, int renormalize, float scale,
+                               void* stream);
+
+/* Rows sorted by expert: ids[rows] (rows = tokens * top_k) -> offsets[experts+1], order[rows] (sorted place -> row, -1
+ * past offsets[experts]), slots[rows] (row -> sorted place, -1 where its id is outside [0, experts)).  Rows of one expert
+ * keep their order. */
+int ftb_expert_plan(const int32_t* ids, int32_t* offsets, int32_t* order, int32_t* slots, int64_t rows, int64_t experts,
+                    void* stream);
+
+/* For every sorted place p of expert e: out[p,n] = epilogue of ftb_linear (no residual) over x-row . w[e]^T + bias[e].
+ * gather = 1: x is [rows / top_k, k] and place p reads row order[p] / top_k; gather = 0: x is [rows, k], sorted.
+ * w[experts, n or 2n, k], bias[experts, n or 2n].  Places past offsets[experts] are left as they were in out and preact.
+ * Knobs as for ftb_linear, without split_k. */
+int ftb_expert_linear(int dtype, const void* x, const void* w, const void* bias, const int32_t* offsets,
+                      const int32_t* order, void* out, void* preact, int64_t rows, int64_t top_k, int64_t experts,
+                      int64_t n, int64_t k, int activation, int gated, int gather, const ftb_config* cfg, int* status,
+                      void* stream);
+/* Gradients: dx[rows,k] by sorted place (a gathered x gets the sum of its places by ftb_expert_combine without weights;
+ * places past offsets[experts] are left as they were), dw[experts, n or 2n, k], db[experts, n or 2n] (zeros for an expert
+ * without rows).  Each may be null. */
+size_t ftb_expert_linear_backward_workspace_bytes(int64_t rows, int64_t experts, int64_t n, int64_t k, int gated);
+int ftb_expert_linear_backward(int dtype, const void* x, const void* w, const int32_t* offsets, const int32_t* order,
+                               const void* dy, const void* preact, void* dx, void* dw, void* db, int64_t rows,
+                               int64_t top_k, int64_t experts, int64_t n, int64_t k, int activation, int gated, int gather,
+                               void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/* out[tokens,n] = residual[tokens,n] + sum over j of weights[token,j] * y[slots[token*top_k+j], n]; dropped rows add
+ * nothing; residual and weights (then all ones) may be null; residual may be `out` itself. */
+int ftb_expert_combine(int dtype, const void* y, const int32_t* slots, const float* weights, const void* residual,
+                       void* out, int64_t tokens, int64_t top_k, int64_t n, void* stream);
+/* dy[place,n] = weights[row] * dout[row / top_k, n] and dweights[row] = dout[row / top_k] . y[place] (0 for a dropped
+ * row).  Either result may be null; y is read for dweights only; places that no row has are left as they were. */
+int ftb_expert_combine_backward(int dtype, const void* dout, const void* y, const int32_t* slots, const float* weights,
+                                void* dy, float* dweights, int64_t tokens, int64_t top_k, int64_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
