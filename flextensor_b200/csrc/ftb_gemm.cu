@@ -2,6 +2,7 @@
 // resolution/validation and the C-ABI launchers for GEMM fp32, batched GEMM bf16,
 // GEMM int8 and conv2d (implicit GEMM).
 #include "ftb_host.h"
+#include "ftb_tmap.h"
 #include "ftb_umma_kernel.cuh"
 #include "ftb_conv_slab_kernel.cuh"
 
@@ -29,9 +30,9 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // rank-`rank` tiled map (128-byte swizzle unless told otherwise); strides in bytes for dims 1..rank-1.
-static int make_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base,
-                     const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                     const uint32_t* elem_strides, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+int make_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+              const uint64_t* strides_bytes, const uint32_t* box, const uint32_t* elem_strides,
+              CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (!fn) return FTB_E_CUDA;
   CUresult r = fn(map, dt, rank, const_cast<void*>(base), dims, strides_bytes, box, elem_strides,

@@ -628,3 +628,100 @@ def test_expert_refusals(B):
     with pytest.raises(ValueError):
         B.expert_combine_backward(torch.empty(6, 32, device="cuda", dtype=torch.bfloat16), plan,
                                   dweights=torch.empty(6, 2, device="cuda"))
+
+
+# ---------------------------------------------------------------- every variant of the tensor-core kernel
+CFGS = [{"tile_n": 16}, {"tile_n": 32}, {"tile_n": 64, "split_k": 1}, {"tile_n": 128}, {"cluster": 2, "tile_n": 128},
+        {"cluster": 2, "tile_n": 256}, {"tile_n": 16, "split_k": 2}, {"tile_n": 32, "split_k": 4}, {"tile_n": 64, "split_k": 8},
+        {"stages": 2}, {"tile_n": 64, "stages": 2, "split_k": 8}, {"cluster": 2}, {"split_k": 4}]
+
+
+@pytest.mark.parametrize("cfg", CFGS, ids=lambda c: "-".join("%s%d" % i for i in c.items()))
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_knobs(B, status, cfg, gated):
+    for t, n, k in ((1, 130, 264), (75, 200, 520), (300, 700, 200)):
+        x, w = rand(1, t, k), rand(2, n * (2 if gated else 1), k, scale=k ** -0.5)
+        b, r = rand(3, w.shape[0]), rand(4, t, n)
+        out = torch.full((t, n), float("nan"), device="cuda", dtype=torch.bfloat16)
+        B.linear(x, w, out, bias=b, residual=r, activation="gelu_tanh", gated=gated, cfg=cfg, status=status)
+        want, tol, _, _ = forward64(x, w, b, r, "gelu_tanh", gated)
+        bounded(out, want, tol + store(want, torch.bfloat16), "%s %s" % (cfg, (t, n, k)))
+        again = torch.empty_like(out)
+        B.linear(x, w, again, bias=b, residual=r, activation="gelu_tanh", gated=gated, cfg=cfg, status=status)
+        assert torch.equal(out, again)  # no order of sums depends on timing
+
+
+@pytest.mark.parametrize("cfg", [c for c in CFGS if c.get("split_k", 1) == 1], ids=lambda c: "-".join("%s%d" % i for i in c.items()))
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+def test_expert_linear_knobs(B, status, cfg, gated, gather):
+    t, k, e, n, width = 210, 3, 5, 330, 200
+    ids = make_ids(t, k, e, drop=0.1)
+    plan = planned(B, ids, e)
+    offsets, order, _ = plan64(ids, e)
+    x, w = rand(1, t if gather else t * k, width), rand(2, e, n * (2 if gated else 1), width, scale=width ** -0.5)
+    out = torch.full((t * k, n), 7.0, device="cuda", dtype=torch.bfloat16)
+    B.expert_linear(x, w, plan, out, activation="silu", gated=gated, gather=gather, cfg=cfg, status=status)
+    used = offsets[-1]
+    src = x[torch.tensor(order[:used], device="cuda") // k] if gather else x[:used]
+    for i in range(e):
+        a, c = offsets[i], offsets[i + 1]
+        want, tol, _, _ = forward64(src[a:c], w[i], None, None, "silu", gated)
+        bounded(out[a:c], want, tol + store(want, torch.bfloat16), "expert %d" % i)
+    assert (out[used:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,n,k,gated", [(1300, 2600, 136, False), (1025, 1111, 72, True), (520, 6000, 64, False), (2100, 600, 328, True)])
+def test_linear_large(B, status, dtype, t, n, k, gated):
+    """Sizes whose defaults are the pair tiles, forward and backward."""
+    wide = 2 * n if gated else n
+    x, w, b = rand(1, t, k, dtype=dtype), rand(2, wide, k, scale=k ** -0.5, dtype=dtype), rand(3, wide, dtype=dtype)
+    out, z = torch.empty(t, n, device="cuda", dtype=dtype), torch.empty(t, wide, device="cuda", dtype=dtype)
+    B.linear(x, w, out, bias=b, activation="silu", gated=gated, preact=z, status=status)
+    want, tol, z64, ez = forward64(x, w, b, None, "silu", gated)
+    bounded(out, want, tol + store(want, dtype), "out")
+    bounded(z, z64, ez + store(z64, dtype), "preact")
+    dy = rand(4, t, n, dtype=dtype)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    ws = torch.empty(B.linear_backward_workspace_bytes(t, n, k, gated), dtype=torch.uint8, device="cuda")
+    B.linear_backward(x, w, dy, dx=dx, dweight=dw, dbias=db, preact=z, activation="silu", gated=gated, workspace=ws, status=status)
+    want = gradients64(x, w, dy, z, "silu", gated)
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        bounded(got, *want[name], name)
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+def test_expert_large(B, status, gather, gated):
+    """Groups long enough for the pair tiles, one of them empty and one of a single row."""
+    t, k, e, n, width = 1700, 2, 4, 1300, 520
+    gen = torch.Generator().manual_seed(0)
+    ids = torch.randint(0, 2, (t, k), generator=gen, dtype=torch.int32)
+    ids[5, 0] = 3
+    ids[-40:] = -1
+    ids = ids.cuda()
+    plan = planned(B, ids, e)
+    offsets, order, _ = plan64(ids, e)
+    used, rows, wide = offsets[-1], t * k, n * (2 if gated else 1)
+    x, w = rand(1, t if gather else rows, width), rand(2, e, wide, width, scale=width ** -0.5)
+    out, z = torch.zeros(rows, n, device="cuda", dtype=torch.bfloat16), torch.zeros(rows, wide, device="cuda", dtype=torch.bfloat16)
+    B.expert_linear(x, w, plan, out, activation="gelu", gated=gated, gather=gather, preact=z, status=status)
+    src = x[torch.tensor(order[:used], device="cuda") // k] if gather else x[:used]
+    dy = rand(3, rows, n)
+    dx, dw, db = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16), torch.empty_like(w), torch.empty(e, wide, device="cuda", dtype=torch.bfloat16)
+    ws = torch.empty(B.expert_linear_backward_workspace_bytes(plan, n, width, gated), dtype=torch.uint8, device="cuda")
+    B.expert_linear_backward(x, w, plan, dy, dx=dx, dweight=dw, dbias=db, preact=z, activation="gelu", gated=gated, gather=gather,
+                             workspace=ws, status=status)
+    for i in range(e):
+        a, c = offsets[i], offsets[i + 1]
+        if a == c:
+            assert not dw[i].any() and not db[i].any()
+            continue
+        want, tol, z64, ez = forward64(src[a:c], w[i], None, None, "gelu", gated)
+        bounded(out[a:c], want, tol + store(want, torch.bfloat16), "out %d" % i)
+        bounded(z[a:c], z64, ez + store(z64, torch.bfloat16), "preact %d" % i)
+        want = gradients64(src[a:c], w[i], dy[a:c], z[a:c], "gelu", gated)
+        for name, got in (("dx", dx[a:c]), ("dw", dw[i]), ("db", db[i])):
+            bounded(got, *want[name], "%s %d" % (name, i))
+    assert not out[used:].any() and not dx[used:].any()
