@@ -604,7 +604,7 @@ MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
 
 def _element(t, name):
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float16):
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float16) or not t.is_cuda:
         raise TypeError("%s must be a bfloat16 or float16 CUDA tensor" % name)
     return t.dtype
 
@@ -613,6 +613,9 @@ def _fits(t, name, shape, dtype, device):
     """One operand's type, device, layout and shape; its address (None passes through)."""
     if t is None:
         return None
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.shape == shape and
+            t.is_contiguous()):
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA tensor" % name)
     if t.dtype != dtype:
@@ -621,9 +624,7 @@ def _fits(t, name, shape, dtype, device):
         raise ValueError("%s is on %s, the call's other tensors on %s" % (name, t.device, device))
     if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if not t.is_contiguous():
-        raise ValueError("%s must be contiguous" % name)
-    return t.data_ptr()
+    raise ValueError("%s must be contiguous" % name)
 
 
 def _one_of(value, table, what):
@@ -632,23 +633,37 @@ def _one_of(value, table, what):
     return table[value]
 
 
+_entries = {}
+
+
 def _call(entry, device, stream, *args):
     """A launcher on ``device``: its current stream unless one is given."""
+    index = device.index
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        raw = torch._C._cuda_getCurrentRawStream(index)
     elif stream.device != device:
         raise ValueError("the stream belongs to %s, the tensors to %s" % (stream.device, device))
-    if torch.cuda.current_device() == device.index:
-        rc = getattr(lib(), entry)(*args, stream.cuda_stream)
+    else:
+        raw = stream.cuda_stream
+    func = _entries.get(entry)
+    if func is None:
+        func = _entries[entry] = getattr(lib(), entry)
+    if torch._C._cuda_getDevice() == index:
+        rc = func(*args, raw)
     else:
         with torch.cuda.device(device):
-            rc = getattr(lib(), entry)(*args, stream.cuda_stream)
+            rc = func(*args, raw)
     if rc:
         raise FtbError(rc, entry)
 
 
 def _status_of(status, device):
     return None if status is None else _fits(status, "status", (1,), torch.int32, device)
+
+
+def _logits(t):
+    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES or not t.is_cuda:
+        raise TypeError("logits must be a float32, bfloat16 or float16 CUDA tensor")
 
 
 def _matrix(t, name, dims):
@@ -736,8 +751,7 @@ def route_experts(logits, ids, weights, bias=None, scoring="softmax", groups=1, 
     only the ``top_groups`` best runs stay.  ``renormalize``: weights are divided by their sum; then times ``scale``.
     A logit of -inf or NaN has score 0.  At most 1024 experts, top_k 32, 32 groups.
     """
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in DTYPES:
-        raise TypeError("logits must be a float32, bfloat16 or float16 CUDA tensor")
+    _logits(logits)
     kind = _one_of(scoring, SCORINGS, "scoring")
     tokens, experts = _matrix(logits, "logits", 2)
     top_k = _matrix(ids, "ids", 2)[1]
@@ -758,8 +772,7 @@ def route_experts(logits, ids, weights, bias=None, scoring="softmax", groups=1, 
 def route_experts_backward(logits, ids, dweights, dlogits, scoring="softmax", renormalize=True, scale=1.0, stream=None):
     """dlogits[T,E] (type of the logits) from dweights[T,top_k] (float32) of ``route_experts`` with the same settings;
     the choice itself has no gradient.  An id outside [0, E) adds nothing."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in DTYPES:
-        raise TypeError("logits must be a float32, bfloat16 or float16 CUDA tensor")
+    _logits(logits)
     kind = _one_of(scoring, SCORINGS, "scoring")
     tokens, experts = _matrix(logits, "logits", 2)
     top_k = _matrix(ids, "ids", 2)[1]

@@ -34,6 +34,8 @@ __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict
   int* mine = hist + warp * experts;
   for (int e = lane; e < experts; e += 32) mine[e] = 0;
   __syncwarp();
+  grid_dependency_wait();
+  grid_launch_dependents();
   for (long long r = r0; r < r1; r += 32) {
     int key = r + lane < r1 ? ids[r + lane] : -1;
     if (key >= experts) key = -1;
@@ -110,9 +112,9 @@ __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict
 
 static int launch_plan(const int* ids, int* offsets, int* order, int* slots, int64_t rows, int64_t experts,
                        cudaStream_t stream) {
-  // one CTA up to 4096 rows (128 rows a warp); above that eight share them
-  const int ctas = rows > 4096 ? kPlanCtas : 1;
-  int64_t warps = ceil_div64(rows, static_cast<int64_t>(ctas) * 64);
+  // one CTA up to 1024 rows (32 rows a warp); above that eight share them
+  const int ctas = rows > 1024 ? kPlanCtas : 1;
+  int64_t warps = ceil_div64(rows, static_cast<int64_t>(ctas) * 32);
   if (warps < 4) warps = 4;
   if (warps > 32) warps = 32;
   const size_t smem = static_cast<size_t>(warps + 3) * experts * sizeof(int);
@@ -129,23 +131,8 @@ static int launch_plan(const int* ids, int* offsets, int* order, int* slots, int
       done[dev] = true;
     }
   }
-  cudaLaunchConfig_t lc;
-  memset(&lc, 0, sizeof(lc));
-  lc.gridDim = dim3(static_cast<unsigned>(ctas));
-  lc.blockDim = dim3(static_cast<unsigned>(warps * 32));
-  lc.dynamicSmemBytes = smem;
-  lc.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  lc.attrs = attr;
-  lc.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&lc, expert_plan_kernel, ids, offsets, order, slots, static_cast<int>(rows),
-                                           static_cast<int>(experts));
-  count_launch();
-  return launch_status(e);
+  return launch_overlapped(expert_plan_kernel, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(warps * 32)), smem,
+                           ctas, stream, ids, offsets, order, slots, static_cast<int>(rows), static_cast<int>(experts));
 }
 
 // ------------------------------------------------------------------ weighted sum of a token's rows
@@ -155,6 +142,8 @@ __global__ void __launch_bounds__(128)
 expert_combine_kernel(const uint16_t* __restrict__ y, const int* __restrict__ slots, const float* __restrict__ weights,
                       const uint16_t* residual, uint16_t* out, int top_k, long long n, long long rows, int blocks_n,
                       int f16_i) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const bool f16 = f16_i != 0;
   const long long t = blockIdx.x / blocks_n;
   const long long c = (static_cast<long long>(blockIdx.x % blocks_n) * 128 + threadIdx.x) * VEC;
@@ -207,6 +196,8 @@ __global__ void __launch_bounds__(256)
 expert_combine_backward_kernel(const uint16_t* __restrict__ dout, const uint16_t* __restrict__ y,
                                const int* __restrict__ slots, const float* __restrict__ weights, uint16_t* __restrict__ dy,
                                float* __restrict__ dweights, long long rows, int top_k, long long n, int f16_i) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const bool f16 = f16_i != 0;
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -291,10 +282,8 @@ int ftb_expert_combine(int dtype, const void* y, const int32_t* slots, const flo
   uint16_t* ov = static_cast<uint16_t*>(out);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int k = static_cast<int>(top_k), f16 = dtype == FTB_F16;
-  if (vec) expert_combine_kernel<8><<<grid, 128, 0, s>>>(yv, slots, weights, rv, ov, k, n, tokens * top_k, static_cast<int>(blocks_n), f16);
-  else expert_combine_kernel<1><<<grid, 128, 0, s>>>(yv, slots, weights, rv, ov, k, n, tokens * top_k, static_cast<int>(blocks_n), f16);
-  count_launch();
-  return launch_status(cudaSuccess);
+  return launch_overlapped(vec ? expert_combine_kernel<8> : expert_combine_kernel<1>, dim3(grid), dim3(128), 0, 1, s, yv, slots,
+                           weights, rv, ov, k, n, tokens * top_k, static_cast<int>(blocks_n), f16);
 }
 
 int ftb_expert_combine_backward(int dtype, const void* dout, const void* y, const int32_t* slots, const float* weights,
@@ -314,10 +303,9 @@ int ftb_expert_combine_backward(int dtype, const void* dout, const void* y, cons
   uint16_t* d = static_cast<uint16_t*>(dy);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int k = static_cast<int>(top_k), f16 = dtype == FTB_F16;
-  if (vec_ok(n, dout, dweights ? y : nullptr, dy)) expert_combine_backward_kernel<8><<<grid, 256, 0, s>>>(g, yv, slots, weights, d, dweights, rows, k, n, f16);
-  else expert_combine_backward_kernel<1><<<grid, 256, 0, s>>>(g, yv, slots, weights, d, dweights, rows, k, n, f16);
-  count_launch();
-  return launch_status(cudaSuccess);
+  const bool vec = vec_ok(n, dout, dweights ? y : nullptr, dy);
+  return launch_overlapped(vec ? expert_combine_backward_kernel<8> : expert_combine_backward_kernel<1>, dim3(grid), dim3(256), 0, 1,
+                           s, g, yv, slots, weights, d, dweights, rows, k, n, f16);
 }
 
 }  // extern "C"

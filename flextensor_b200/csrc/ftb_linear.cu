@@ -11,12 +11,52 @@ namespace ftb {
 constexpr int kDzRows = 8;
 
 template <int VEC>
+struct DzIn {
+  uint32_t d[(VEC + 1) / 2], a[(VEC + 1) / 2], u[(VEC + 1) / 2];
+};
+
+template <int VEC>
+__device__ __forceinline__ void dz_read(uint32_t (&w)[(VEC + 1) / 2], const uint16_t* p) {
+  if constexpr (VEC == 8) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    w[0] = q.x;
+    w[1] = q.y;
+    w[2] = q.z;
+    w[3] = q.w;
+  } else {
+    w[0] = *p;
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void dz_unpack(float (&f)[VEC], const uint32_t (&w)[(VEC + 1) / 2], bool f16) {
+  if constexpr (VEC == 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = unpack16(w[i], f16);
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  } else {
+    f[0] = from16(static_cast<uint16_t>(w[0]), f16);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void dz_write(uint16_t* p, const float (&f)[VEC], bool f16) {
+  if constexpr (VEC == 8)
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack16(f[0], f[1], f16), pack16(f[2], f[3], f16), pack16(f[4], f[5], f16), pack16(f[6], f[7], f16));
+  else
+    *p = to16(f[0], f16);
+}
+
+template <int VEC, bool GATED>
 __global__ void __launch_bounds__(256)
 linear_dz_kernel(const uint16_t* __restrict__ dy, const uint16_t* __restrict__ z, uint16_t* __restrict__ dz,
                  long long ldz, float* __restrict__ partial, const int* __restrict__ offsets, long long rows, long long n,
-                 int act, int gated, int f16_i, int chunks) {
+                 int act, int f16_i, int chunks) {
   const bool f16 = f16_i != 0;
   __shared__ float sums[kDzRows][32 * VEC + 1];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int g = blockIdx.z;
   int lo = 0, hi = static_cast<int>(rows);
   if (offsets) group_range(offsets, g, rows, &lo, &hi);
@@ -24,75 +64,57 @@ linear_dz_kernel(const uint16_t* __restrict__ dy, const uint16_t* __restrict__ z
   const long long r0 = lo + static_cast<long long>(blockIdx.y) * per;
   const long long r1 = min(r0 + per, static_cast<long long>(hi));
   const long long c0 = (static_cast<long long>(blockIdx.x) * 32 + threadIdx.x) * VEC;
-  const long long wide = gated ? 2 * n : n;
+  const long long wide = GATED ? 2 * n : n;
   float s0[VEC] = {}, s1[VEC] = {};
   if (c0 < n) {
-    for (long long r = r0 + threadIdx.y; r < r1; r += kDzRows) {
-      float d[VEC], a[VEC], u[VEC];
-      if constexpr (VEC == 8) {
-        const uint4 q = *reinterpret_cast<const uint4*>(dy + r * n + c0);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    // the next row is on its way while this one is worked on
+    DzIn<VEC> next;
+    auto fetch = [&](long long r) {
+      dz_read<VEC>(next.d, dy + r * n + c0);
+      if (z) {
+        dz_read<VEC>(next.a, z + r * wide + c0);
+        if (GATED) dz_read<VEC>(next.u, z + r * wide + n + c0);
+      }
+    };
+    long long r = r0 + threadIdx.y;
+    if (r < r1) fetch(r);
+    for (; r < r1; r += kDzRows) {
+      const DzIn<VEC> in = next;
+      if (r + kDzRows < r1) fetch(r + kDzRows);
+      float d[VEC], g0[VEC];
+      dz_unpack<VEC>(d, in.d, f16);
+      if (z) {
+        float a[VEC], value[VEC], slope[VEC];
+        dz_unpack<VEC>(a, in.a, f16);
+        act_both<VEC>(a, value, slope, act);
+        if constexpr (GATED) {
+          float u[VEC];
+          dz_unpack<VEC>(u, in.u, f16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack16(w[i], f16);
-          d[2 * i] = f.x;
-          d[2 * i + 1] = f.y;
-        }
-        if (z) {
-          const uint4 qa = *reinterpret_cast<const uint4*>(z + r * wide + c0);
-          const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w};
-          uint4 qu = make_uint4(0, 0, 0, 0);
-          if (gated) qu = *reinterpret_cast<const uint4*>(z + r * wide + n + c0);
-          const uint32_t wu[4] = {qu.x, qu.y, qu.z, qu.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 fa = unpack16(wa[i], f16), fu = unpack16(wu[i], f16);
-            a[2 * i] = fa.x;
-            a[2 * i + 1] = fa.y;
-            u[2 * i] = fu.x;
-            u[2 * i + 1] = fu.y;
+          for (int i = 0; i < VEC; ++i) {
+            g0[i] = d[i] * u[i] * slope[i];
+            value[i] *= d[i];
+            s1[i] += value[i];
           }
+          if (dz) dz_write<VEC>(dz + r * ldz + n + c0, value, f16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) g0[i] = d[i] * slope[i];
         }
       } else {
-        d[0] = from16(dy[r * n + c0], f16);
-        if (z) {
-          a[0] = from16(z[r * wide + c0], f16);
-          u[0] = gated ? from16(z[r * wide + n + c0], f16) : 0.0f;
-        }
-      }
-      float g0[VEC], g1[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        g0[i] = d[i];
-        g1[i] = 0.0f;
-        if (gated) {
-          g0[i] = d[i] * u[i] * act_slope(a[i], act);
-          g1[i] = d[i] * act_value(a[i], act);
-        } else if (z) {
-          g0[i] = d[i] * act_slope(a[i], act);
-        }
-        s0[i] += g0[i];
-        s1[i] += g1[i];
+        for (int i = 0; i < VEC; ++i) g0[i] = d[i];
       }
-      if (dz) {
-        // one rounding to the element type: what the two products read
-        if constexpr (VEC == 8) {
-          *reinterpret_cast<uint4*>(dz + r * ldz + c0) =
-              make_uint4(pack16(g0[0], g0[1], f16), pack16(g0[2], g0[3], f16), pack16(g0[4], g0[5], f16), pack16(g0[6], g0[7], f16));
-          if (gated)
-            *reinterpret_cast<uint4*>(dz + r * ldz + n + c0) =
-                make_uint4(pack16(g1[0], g1[1], f16), pack16(g1[2], g1[3], f16), pack16(g1[4], g1[5], f16), pack16(g1[6], g1[7], f16));
-        } else {
-          dz[r * ldz + c0] = to16(g0[0], f16);
-          if (gated) dz[r * ldz + n + c0] = to16(g1[0], f16);
-        }
-      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s0[i] += g0[i];
+      if (dz) dz_write<VEC>(dz + r * ldz + c0, g0, f16);  // one rounding to the element type: what the products read
     }
   }
   if (!partial) return;
   float* row = partial + (static_cast<long long>(g) * chunks + blockIdx.y) * wide;
   const int t = threadIdx.y * 32 + threadIdx.x;
-  for (int half = 0; half < (gated ? 2 : 1); ++half) {
+#pragma unroll
+  for (int half = 0; half < (GATED ? 2 : 1); ++half) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sums[threadIdx.y][threadIdx.x * VEC + i] = half ? s1[i] : s0[i];
@@ -110,6 +132,8 @@ linear_dz_kernel(const uint16_t* __restrict__ dy, const uint16_t* __restrict__ z
 __global__ void __launch_bounds__(256)
 bias_sum_kernel(const float* __restrict__ partial, uint16_t* __restrict__ db, long long wide, long long total, int chunks,
                 int f16) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (t >= total) return;
   const long long g = t / wide, c = t - g * wide;
@@ -194,18 +218,15 @@ static int backward_generic(int dtype, const void* x, const void* w, const int* 
     const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(chunks), static_cast<unsigned>(groups));
     const uint16_t* z = need_z ? static_cast<const uint16_t*>(preact) : nullptr;
     const uint16_t* d = static_cast<const uint16_t*>(dy);
-    if (vec)
-      linear_dz_kernel<8><<<grid, dim3(32, kDzRows), 0, stream>>>(d, z, write_dz ? dz : nullptr, ldz, partial, offsets, rows, n, activation, gated, f16, chunks);
-    else
-      linear_dz_kernel<1><<<grid, dim3(32, kDzRows), 0, stream>>>(d, z, write_dz ? dz : nullptr, ldz, partial, offsets, rows, n, activation, gated, f16, chunks);
-    count_launch();
-    int e = launch_status(cudaSuccess);
+    auto kern = vec ? (gated ? linear_dz_kernel<8, true> : linear_dz_kernel<8, false>)
+                    : (gated ? linear_dz_kernel<1, true> : linear_dz_kernel<1, false>);
+    int e = launch_overlapped(kern, grid, dim3(32, kDzRows), 0, 1, stream, d, z, write_dz ? dz : nullptr, ldz, partial, offsets,
+                              rows, n, activation, f16, chunks);
     if (e) return e;
     if (db) {
       const int64_t total = groups * wide;
-      bias_sum_kernel<<<static_cast<unsigned>(ceil_div64(total, 256)), 256, 0, stream>>>(partial, static_cast<uint16_t*>(db), wide, total, chunks, f16);
-      count_launch();
-      e = launch_status(cudaSuccess);
+      e = launch_overlapped(bias_sum_kernel, dim3(static_cast<unsigned>(ceil_div64(total, 256))), dim3(256), 0, 1, stream,
+                            partial, static_cast<uint16_t*>(db), wide, total, chunks, f16);
       if (e) return e;
     }
   }

@@ -11,6 +11,8 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinArgs p) {
   constexpr int T = 64, TK = 16, SUBS = GATED ? 2 : 1;
   __shared__ float As[SUBS][TK][T + 1];
   __shared__ float Bs[TK][T + 1];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const bool f16 = p.f16 != 0;
   const int g = blockIdx.z;
   int lo = 0, hi = 0;
@@ -114,10 +116,7 @@ int launch_linear_simt(const LinArgs& p, cudaStream_t stream) {
   const int64_t gx = ceil_div64(p.I, 64);
   if (gx > 0x7fffffff) return FTB_E_TOO_LARGE;
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy), static_cast<unsigned>(p.groups));
-  if (p.gated) linear_simt_kernel<true><<<grid, 256, 0, stream>>>(p);
-  else linear_simt_kernel<false><<<grid, 256, 0, stream>>>(p);
-  count_launch();
-  return launch_status(cudaSuccess);
+  return launch_overlapped(p.gated ? linear_simt_kernel<true> : linear_simt_kernel<false>, grid, dim3(256), 0, 1, stream, p);
 }
 
 }  // namespace ftb

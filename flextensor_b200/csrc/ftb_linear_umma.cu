@@ -43,7 +43,13 @@ struct LinUmma {
   uint32_t idesc;
   uint32_t a_lbo, b_lbo, a_kadv, b_kadv;
   int oob_a, oob_b;      // a row past the gathered tensors
+  int vec;               // rows of out, residual and preact start on 16 bytes
   int* status;
+};
+
+// Tiled maps of the operands, and maps whose boxes are one row high for rows fetched by number.
+struct LinMaps {
+  CUtensorMap a, b, a_rows, b_rows;
 };
 
 struct LinTile {
@@ -111,56 +117,145 @@ __device__ __forceinline__ void act_values(float (&v)[NC], int act) {
   }
 }
 
-// bias, activation, gate, residual and the stores of `NC` neighbouring tokens of one feature; `at` is its element of the
-// first token in out and residual, `zat` in preact.
-template <int NC, bool GATED>
-__device__ __forceinline__ void lin_finish(const LinArgs& q, float (&v)[NC], float (&u)[NC], float b0, float b1,
-                                           long long at, long long zat, int valid) {
+// The epilogue of 16 columns (tokens) by one warp, whose lanes hold 32 neighbouring features.  The arithmetic runs as
+// the accumulator lies, a feature per lane.  Where every row of the results starts on 16 bytes (`vec`) a warp then turns
+// its 16 x 32 values round through 2.25 KB of shared memory and a lane loads and stores eight features of a token at a
+// time: about a quarter of the instructions of 2-byte accesses, which bound the epilogue (GELU with bias, residual and
+// preact at 1237 x 2051 x 1000: 10 us of 21 before).  Rows of other pitches keep the 2-byte accesses, 64 contiguous
+// bytes per warp.
+constexpr int kCols = 16;          // columns a thread holds at a time
+constexpr int kTurnPitch = 36;     // floats between two tokens: a lane's 16-byte reads meet no bank twice
+constexpr int kTurnFloats = kCols * kTurnPitch;
+
+struct WarpCols {
+  float* turn;        // this warp's staging
+  int lane;
+  bool live;          // the lane's feature exists
+  bool live8;         // so do the eight features that the lane moves in the turned layout
+  int valid;          // columns that are tokens of this tile
+};
+
+// Reads the residual before the sums are ready: turned, 2 x 8 features; else 16 tokens of the lane's feature.
+__device__ __forceinline__ void lin_residual(const LinArgs& q, bool vec, const WarpCols& w, uint32_t (&res)[kCols],
+                                             const uint16_t* first) {
+  if (vec) {
+    const uint16_t* r = first + (w.lane >> 2) * q.ldo + (w.lane & 3) * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (w.live8 && (w.lane >> 2) + 8 * h < w.valid) x = *reinterpret_cast<const uint4*>(r + 8 * h * q.ldo);
+      res[4 * h] = x.x;
+      res[4 * h + 1] = x.y;
+      res[4 * h + 2] = x.z;
+      res[4 * h + 3] = x.w;
+    }
+  } else {
+    const uint16_t* r = first + w.lane;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      res[c] = w.live && c < w.valid ? *r : 0u;
+      r += q.ldo;
+    }
+  }
+}
+
+// Rounds and stores the warp's 16 x 32 values; `first` is the element of column 0 and lane 0, `res` null or the residual.
+__device__ __forceinline__ void lin_store(bool vec, bool f16, const WarpCols& w, float (&v)[kCols], uint16_t* first,
+                                          long long pitch, const uint32_t* res) {
+  if (vec) {
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) w.turn[c * kTurnPitch + w.lane] = v[c];
+    __syncwarp();
+    const int tok = w.lane >> 2, oct = (w.lane & 3) * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 a = *reinterpret_cast<const float4*>(w.turn + (tok + 8 * h) * kTurnPitch + oct);
+      const float4 b = *reinterpret_cast<const float4*>(w.turn + (tok + 8 * h) * kTurnPitch + oct + 4);
+      float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      if (res) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 r = unpack16(res[4 * h + e], f16);
+          x[2 * e] += r.x;
+          x[2 * e + 1] += r.y;
+        }
+      }
+      if (w.live8 && tok + 8 * h < w.valid)
+        *reinterpret_cast<uint4*>(first + (tok + 8 * h) * pitch + oct) =
+            make_uint4(pack16(x[0], x[1], f16), pack16(x[2], x[3], f16), pack16(x[4], x[5], f16), pack16(x[6], x[7], f16));
+    }
+  } else {
+    uint16_t* o = first + w.lane;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      float x = v[c];
+      if (res) x += from16(static_cast<uint16_t>(res[c]), f16);
+      if (w.live && c < w.valid) *o = to16(x, f16);
+      o += pitch;
+    }
+  }
+}
+
+template <bool GATED>
+__device__ __forceinline__ void lin_finish(const LinArgs& q, bool vec, const WarpCols& w, float (&v)[kCols],
+                                           float (&u)[kCols], const uint32_t (&res)[kCols], float b0, float b1,
+                                           uint16_t* out, uint16_t* preact) {
   const bool f16 = q.f16 != 0;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
+  for (int c = 0; c < kCols; ++c) {
     v[c] += b0;
     if constexpr (GATED) u[c] += b1;
   }
   if (q.preact) {
-    uint16_t* z = q.preact + zat;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      if (c < valid) {
-        *z = to16(v[c], f16);
-        if constexpr (GATED) z[q.I] = to16(u[c], f16);
-      }
-      z += q.ldp;
-    }
+    lin_store(vec, f16, w, v, preact, q.ldp, nullptr);
+    if constexpr (GATED) lin_store(vec, f16, w, u, preact + q.I, q.ldp, nullptr);
   }
-  act_values<NC>(v, q.act);
+  act_values<kCols>(v, q.act);
   if constexpr (GATED) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) v[c] *= u[c];
+    for (int c = 0; c < kCols; ++c) v[c] *= u[c];
   }
-  if (q.residual) {
-    const uint16_t* r = q.residual + at;
-    uint16_t res[NC];
+  lin_store(vec, f16, w, v, out, q.ldo, q.residual ? res : nullptr);
+}
+
+// The same for four neighbouring features of one token (after a split reduction).
+template <bool GATED>
+__device__ __forceinline__ void lin_finish4(const LinArgs& q, float (&v)[4], float (&u)[4], const float (&b0)[4],
+                                            const float (&b1)[4], const uint16_t (&res)[4], long long i, long long row) {
+  const bool f16 = q.f16 != 0;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      res[c] = c < valid ? *r : 0;
-      r += q.ldo;
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) v[c] += from16(res[c], f16);
+  for (int e = 0; e < 4; ++e) {
+    v[e] += b0[e];
+    if constexpr (GATED) u[e] += b1[e];
   }
-  uint16_t* out = q.out + at;
+  if (q.preact) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (c < valid) *out = to16(v[c], f16);
-    out += q.ldo;
+    for (int e = 0; e < 4; ++e)
+      if (i + e < q.I) {
+        q.preact[row * q.ldp + i + e] = to16(v[e], f16);
+        if constexpr (GATED) q.preact[row * q.ldp + q.I + i + e] = to16(u[e], f16);
+      }
+  }
+  act_values<4>(v, q.act);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (GATED) v[e] *= u[e];
+    if (q.residual) v[e] += from16(res[e], f16);
+  }
+  uint16_t* out = q.out + row * q.ldo + i;
+  if (i + 3 < q.I && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack16(v[0], v[1], f16), pack16(v[2], v[3], f16));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < q.I) out[e] = to16(v[e], f16);
   }
 }
 
 template <bool PAIR, int FORM, int EPI, bool SPLIT>
 __global__ void __launch_bounds__(128 + 32 * EPI, EPI == 4 ? 2 : 1)
-linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ LinUmma p) {
+linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinUmma p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kLinStages];
   __shared__ __align__(8) uint64_t bar_empty[kLinStages];
@@ -169,6 +264,7 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int tstart[FTB_MAX_EXPERTS + 1];
+  __shared__ int4 row_quads[2][16];  // rows of the copies that each loader warp issues
   constexpr int SUBS = FORM == FORM_PLAIN ? 1 : 2;
   static_assert(!SPLIT || (!PAIR && FORM != FORM_WIDE && EPI == 4), "the reduction is split in single-CTA tiles only");
 
@@ -194,8 +290,8 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
     fence_mbar_init();
     fence_proxy_async_smem();
-    prefetch_tmap(&map_a);
-    prefetch_tmap(&map_b);
+    prefetch_tmap(&maps.a);
+    prefetch_tmap(&maps.b);
   }
   if (warp == 1) {
     if constexpr (PAIR) {
@@ -207,6 +303,7 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
   }
   if (warp == 3 && mode == LIN_ROWS) {
+    grid_dependency_wait();
     // token tiles before each group
     int base = 0;
     for (int g0 = 0; g0 < p.q.groups; g0 += 32) {
@@ -232,119 +329,148 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   if constexpr (PAIR) cluster_sync_all();  // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  grid_launch_dependents();  // tensor memory is held: a successor's CTA on this SM cannot take it first
+  grid_dependency_wait();
 
   const int total = mode == LIN_ROWS ? tstart[p.q.groups] * p.tiles_i : p.q.groups * p.tiles_i * p.tiles_j;
   const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
   const uint32_t tfull0 = smem_u32(&bar_tfull[0]), tempty0 = smem_u32(&bar_tempty[0]);
   const uint32_t slot_stride = FORM == FORM_WIDE ? static_cast<uint32_t>(p.bn) : static_cast<uint32_t>(p.bn) * SUBS;
 
-  if (warp == 0) {
+  // Rows by number: tokens of a group (gather_j), or places of a reduction whose operand is not sorted or whose last
+  // block ends inside it (gather_k).  One thread gets a gather4 out about every 25 ns, so two warps share them.
+  const bool gather_j = mode == LIN_ROWS && p.q.gather_div != 0;
+  const bool gather_k = mode == LIN_REDUCE;
+  if (warp == 0 || (warp == 3 && (gather_j || gather_k))) {
     // ------------------------------------------------------------ producer
-    const bool gather_j = mode == LIN_ROWS && p.q.gather_div != 0;
-    const bool gather_k = mode == LIN_REDUCE;
-    const bool gather = gather_j || gather_k;
-    const unsigned takers = gather ? 0xffffffffu : 1u;  // lanes of this loop
-    if (lane == 0 || gather) {
-      const uint32_t tx = stage_bytes;
-      const uint32_t sig0 = PAIR ? map_to_cta(full0, 0) : full0;
-      uint32_t s = 0, ph = 0, sa = smem_base;
-      bool ok = true;
-      for (int t = unit; t < total && ok; t += units) {
-        const LinTile c = lin_tile(p, tstart, t);
-        const int blocks = lin_blocks(p, c);
-        const int per = SPLIT ? (blocks + p.split - 1) / p.split : blocks;
-        const int kb0 = SPLIT ? static_cast<int>(rank) * per : 0, kb1 = min(blocks, kb0 + per);
-        const int f0 = c.ti * p.feat + static_cast<int>(rank) * (PAIR ? 128 : 0);
-        const int j0 = c.tj * p.bn + static_cast<int>(rank) * (PAIR ? p.bj : 0);
-        int row[4] = {};
-        if (gather_j && lane * 4 < p.bj) {
+    const int part = warp == 3 ? 1 : 0;
+    const uint32_t tx = stage_bytes;
+    const uint32_t sig0 = PAIR ? map_to_cta(full0, 0) : full0;
+    int4* quads = row_quads[part];
+    uint32_t s = 0, ph = 0, sa = smem_base;
+    bool ok = true;
+    for (int t = unit; t < total && ok; t += units) {
+      const LinTile c = lin_tile(p, tstart, t);
+      const int blocks = lin_blocks(p, c);
+      const int per = SPLIT ? (blocks + p.split - 1) / p.split : blocks;
+      const int kb0 = SPLIT ? static_cast<int>(rank) * per : 0, kb1 = min(blocks, kb0 + per);
+      const int f0 = c.ti * p.feat + static_cast<int>(rank) * (PAIR ? 128 : 0);
+      const int j0 = c.tj * p.bn + static_cast<int>(rank) * (PAIR ? p.bj : 0);
+      const int half = p.bj >> 3;  // gather_j: quads of four rows per loader warp
+      if (gather_j) {
+        __syncwarp();
+        if (lane < half) {
+          int row[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = j0 + lane * 4 + e;
+            const int j = j0 + (part * half + lane) * 4 + e;
             const long long r = j < c.cnt ? gathered_row(p.q, c.lo + j) : -1;
             row[e] = r >= 0 ? static_cast<int>(r) : p.oob_b;
           }
+          quads[lane] = make_int4(row[0], row[1], row[2], row[3]);
         }
-        for (int kb = kb0; kb < kb1; ++kb) {
-          int ra[4], rb[4];
-          if (gather_k) {
-            // this lane's four places of the block: 16 lanes cover its 64
+        __syncwarp();
+      }
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const bool tail = gather_k && (kb + 1) * kKBlock > c.cnt;   // the block ends past the group
+        const bool rows_a = gather_k && (tail || p.q.gather_div != 0), rows_b = tail;
+        if (rows_a) {
+          // quads 0..7: this warp's half of the block's places in A, 8..15: in B
+          __syncwarp();
+          if (lane < 16) {
+            int row[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int k = kb * kKBlock + (lane & 15) * 4 + e;
-              const long long r = k < c.cnt ? gathered_row(p.q, c.lo + k) : -1;
-              ra[e] = r >= 0 ? static_cast<int>(r) : p.oob_a;
-              rb[e] = k < c.cnt ? c.lo + k : p.oob_b;
+              const int k = kb * kKBlock + (part * 8 + (lane & 7)) * 4 + e;
+              if (lane < 8) {
+                const long long r = k < c.cnt ? gathered_row(p.q, c.lo + k) : -1;
+                row[e] = r >= 0 ? static_cast<int>(r) : p.oob_a;
+              } else {
+                row[e] = k < c.cnt ? c.lo + k : p.oob_b;
+              }
             }
+            quads[lane] = make_int4(row[0], row[1], row[2], row[3]);
           }
-          const bool free = mbar_wait(empty0 + 8 * s, ph ^ 1u, &abort_flag);
-          if (!__all_sync(takers, free)) {
-            if (lane == 0) {
-              atomicOr(p.status, FTB_DEV_WAIT_EMPTY);
-              abort_flag = 1;
-            }
-            ok = false;
-            break;
+          __syncwarp();
+        }
+        if (lane == 0) {
+          ok = mbar_wait(empty0 + 8 * s, ph ^ 1u, &abort_flag);
+          if (!ok) {
+            atomicOr(p.status, FTB_DEV_WAIT_EMPTY);
+            abort_flag = 1;
           }
+        }
+        if (lane == 0 && ok) {
           const uint32_t full = sig0 + 8 * s, sb = sa + SUBS * kSubBytes;
-          const int kc = kb * kKBlock;
-          if (lane == 0 && rank * (PAIR ? 1u : 0u) == 0u) mbar_expect_tx(full0 + 8 * s, PAIR ? 2 * tx : tx);
-          if (gather_k) {
-            __syncwarp();
-            const int box = lane >> 4;
-            const uint32_t at = static_cast<uint32_t>(lane & 15) * 512u;
-#pragma unroll
-            for (int sub = 0; sub < SUBS; ++sub) {
-              const uint32_t dst = sa + sub * kSubBytes + box * 8192u + at;
-              const int col = f0 + sub * p.sub_off + box * 64;
-              if constexpr (PAIR) tma_gather4_pair(dst, &map_a, full, col, ra[0], ra[1], ra[2], ra[3]);
-              else tma_gather4(dst, &map_a, full, col, ra[0], ra[1], ra[2], ra[3]);
-            }
-            if (box * 64 < p.bj) {
-              if constexpr (PAIR) tma_gather4_pair(sb + box * 8192u + at, &map_b, full, j0 + box * 64, rb[0], rb[1], rb[2], rb[3]);
-              else tma_gather4(sb + box * 8192u + at, &map_b, full, j0 + box * 64, rb[0], rb[1], rb[2], rb[3]);
-            }
-          } else {
-            if (lane == 0) {
+          const int kc = gather_k ? c.lo + kb * kKBlock : kb * kKBlock;
+          if (part == 0) {
+            if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR ? 2 * tx : tx);
+            if (!rows_a) {
 #pragma unroll
               for (int sub = 0; sub < SUBS; ++sub) {
                 const uint32_t dst = sa + sub * kSubBytes;
-                const int f = f0 + sub * p.sub_off;
+                const int f = f0 + sub * p.sub_off, g = gather_k ? 0 : c.g;
                 if (p.q.a_mn) {
 #pragma unroll
                   for (int b = 0; b < 2; ++b) {
-                    if constexpr (PAIR) tma_load_3d_pair(dst + b * 8192u, &map_a, full, f + b * 64, kc, c.g);
-                    else tma_load_3d(dst + b * 8192u, &map_a, full, f + b * 64, kc, c.g);
+                    if constexpr (PAIR) tma_load_3d_pair(dst + b * 8192u, &maps.a, full, f + b * 64, kc, g);
+                    else tma_load_3d(dst + b * 8192u, &maps.a, full, f + b * 64, kc, g);
                   }
                 } else {
-                  if constexpr (PAIR) tma_load_3d_pair(dst, &map_a, full, kc, f, c.g);
-                  else tma_load_3d(dst, &map_a, full, kc, f, c.g);
+                  if constexpr (PAIR) tma_load_3d_pair(dst, &maps.a, full, kc, f, g);
+                  else tma_load_3d(dst, &maps.a, full, kc, f, g);
                 }
               }
-              if (p.q.b_mn) {
+            }
+            if (p.q.b_mn) {
+              if (!rows_b) {
                 for (int b = 0; b * 64 < p.bj; ++b) {
-                  if constexpr (PAIR) tma_load_3d_pair(sb + b * 8192u, &map_b, full, j0 + b * 64, kc, 0);
-                  else tma_load_3d(sb + b * 8192u, &map_b, full, j0 + b * 64, kc, 0);
+                  if constexpr (PAIR) tma_load_3d_pair(sb + b * 8192u, &maps.b, full, j0 + b * 64, kc, 0);
+                  else tma_load_3d(sb + b * 8192u, &maps.b, full, j0 + b * 64, kc, 0);
                 }
-              } else if (!gather_j) {
-                if constexpr (PAIR) tma_load_3d_pair(sb, &map_b, full, kc, c.lo + j0, 0);
-                else tma_load_3d(sb, &map_b, full, kc, c.lo + j0, 0);
               }
+            } else if (!gather_j) {
+              if constexpr (PAIR) tma_load_3d_pair(sb, &maps.b, full, kc, c.lo + j0, 0);
+              else tma_load_3d(sb, &maps.b, full, kc, c.lo + j0, 0);
             }
-            if (gather_j) {
-              __syncwarp();
-              if (lane * 4 < p.bj) {
-                if constexpr (PAIR) tma_gather4_pair(sb + lane * 512u, &map_b, full, kc, row[0], row[1], row[2], row[3]);
-                else tma_gather4(sb + lane * 512u, &map_b, full, kc, row[0], row[1], row[2], row[3]);
+          }
+          if (gather_j) {
+            uint32_t dst = sb + part * half * 512u;
+#pragma unroll 4
+            for (int e = 0; e < half; ++e, dst += 512u) {
+              const int4 r = quads[e];
+              if constexpr (PAIR) tma_gather4_pair(dst, &maps.b_rows, full, kc, r.x, r.y, r.z, r.w);
+              else tma_gather4(dst, &maps.b_rows, full, kc, r.x, r.y, r.z, r.w);
+            }
+          }
+          if (rows_a) {
+            for (int e = 0; e < 8; ++e) {
+              const int4 r = quads[e];
+              const uint32_t at = static_cast<uint32_t>(part * 8 + e) * 512u;
+#pragma unroll
+              for (int b = 0; b < 2 * SUBS; ++b) {
+                const uint32_t dst = sa + b * 8192u + at;
+                const int col = f0 + (b >> 1) * p.sub_off + (b & 1) * 64;
+                if constexpr (PAIR) tma_gather4_pair(dst, &maps.a_rows, full, col, r.x, r.y, r.z, r.w);
+                else tma_gather4(dst, &maps.a_rows, full, col, r.x, r.y, r.z, r.w);
+              }
+              if (rows_b) {
+                const int4 q = quads[8 + e];
+                for (int b = 0; b * 64 < p.bj; ++b) {
+                  if constexpr (PAIR) tma_gather4_pair(sb + b * 8192u + at, &maps.b_rows, full, j0 + b * 64, q.x, q.y, q.z, q.w);
+                  else tma_gather4(sb + b * 8192u + at, &maps.b_rows, full, j0 + b * 64, q.x, q.y, q.z, q.w);
+                }
               }
             }
           }
-          sa += stage_bytes;
-          if (++s == stages) {
-            s = 0;
-            ph ^= 1u;
-            sa = smem_base;
-          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        sa += stage_bytes;
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+          sa = smem_base;
         }
       }
     }
@@ -437,6 +563,18 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                                             static_cast<long long>(p.bn)));
       const long long row0 = (mode == LIN_ROWS ? c.lo : 0) + j0;
       const long long out_base = mode == LIN_REDUCE ? c.g * p.q.out_gs : 0;
+      constexpr bool GATED = FORM == FORM_GATED;
+      const int first = FORM == FORM_WIDE ? 0 : grp * kCols, step = FORM == FORM_WIDE ? kCols : GROUPS * kCols;
+      const bool vec = p.vec != 0, add = !SPLIT && p.q.residual != nullptr;
+      WarpCols w;
+      w.turn = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)) + stages * stage_bytes) + (warp - 4) * kTurnFloats;
+      w.lane = lane;
+      w.live = live;
+      w.live8 = i - lane + (lane & 3) * 8 < p.q.I;
+      const long long i0 = i - lane;  // the warp's first feature
+      uint32_t res[kCols];
+      w.valid = left - first;
+      if (add) lin_residual(p.q, vec, w, res, p.q.residual + out_base + (row0 + first) * p.q.ldo + i0);
       const bool got = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, aph, &abort_flag));
       if (!got) {
         if (lane == 0) {
@@ -453,45 +591,36 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const int per = (lin_blocks(p, c) + p.split - 1) / p.split;
         const bool mine = static_cast<int>(rank) * per < lin_blocks(p, c);
         for (int sub = 0; sub < SUBS; ++sub)
-          for (int c0 = 0; c0 < p.bn; c0 += 16) {
+          for (int c0 = 0; c0 < p.bn && c0 < left; c0 += 16) {
             uint32_t v[16];
             tmem_ld_32x16(d + sub * p.bn + c0, v);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              part[(sub * p.bn + c0 + e) * 128 + quarter * 32 + lane] = mine ? __uint_as_float(v[e]) : 0.0f;
+              if (c0 + e < left) part[(sub * p.bn + c0 + e) * 128 + quarter * 32 + lane] = mine ? __uint_as_float(v[e]) : 0.0f;
           }
         break;  // one tile per cluster
       } else {
-        constexpr bool GATED = FORM == FORM_GATED;
-        const int first = FORM == FORM_WIDE ? 0 : grp, step = FORM == FORM_WIDE ? 1 : GROUPS;
-        if (p.bn >= 32) {
-          for (int c0 = first * 32; c0 < p.bn && c0 < left; c0 += step * 32) {
-            uint32_t rv[32], ru[32];
-            float v[32], u[32];
-            tmem_ld_32x32(d + c0, rv);
-            if constexpr (GATED) tmem_ld_32x32(d + p.bn + c0, ru);
-            tmem_ld_wait();
+        for (int c0 = first; c0 < p.bn && c0 < left; c0 += step) {
+          uint32_t rv[kCols], ru[kCols], now[kCols];
+          float v[kCols], u[kCols];
+          tmem_ld_32x16(d + c0, rv);
+          if constexpr (GATED) tmem_ld_32x16(d + p.bn + c0, ru);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              v[e] = work ? __uint_as_float(rv[e]) : 0.0f;
-              if constexpr (GATED) u[e] = __uint_as_float(ru[e]);
-            }
-            if (live)
-              lin_finish<32, GATED>(p.q, v, u, b0, b1, out_base + (row0 + c0) * p.q.ldo + i, (row0 + c0) * p.q.ldp + i, left - c0);
+          for (int e = 0; e < kCols; ++e) now[e] = res[e];
+          if (add && c0 + step < left) {
+            w.valid = left - c0 - step;
+            lin_residual(p.q, vec, w, res, p.q.residual + out_base + (row0 + c0 + step) * p.q.ldo + i0);
           }
-        } else if (first == 0) {
-          uint32_t rv[16], ru[16];
-          float v[16], u[16];
-          tmem_ld_32x16(d, rv);
-          if constexpr (GATED) tmem_ld_32x16(d + p.bn, ru);
+          w.valid = left - c0;
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < kCols; ++e) {
             v[e] = work ? __uint_as_float(rv[e]) : 0.0f;
             if constexpr (GATED) u[e] = __uint_as_float(ru[e]);
           }
-          if (live) lin_finish<16, GATED>(p.q, v, u, b0, b1, out_base + row0 * p.q.ldo + i, row0 * p.q.ldp + i, left);
+          lin_finish<GATED>(p.q, vec, w, v, u, now, b0, b1, p.q.out + out_base + (row0 + c0) * p.q.ldo + i0,
+                            p.q.preact + (row0 + c0) * p.q.ldp + i0);
         }
         tc_fence_before();
         __syncwarp();
@@ -514,31 +643,58 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       tmem_dealloc(tmem_base, p.tmem_cols);
     }
     __syncwarp();
-    cluster_sync_all();  // every CTA's partial sums are in its shared memory
-    if (unit < total) {
-      const LinTile c = lin_tile(p, tstart, unit);
-      const int f = threadIdx.x & 127;
-      const long long i = static_cast<long long>(c.ti) * p.feat + f;
-      const long long j0 = static_cast<long long>(c.tj) * p.bn;
-      const int left = static_cast<int>(min(p.q.J - j0, static_cast<long long>(p.bn)));
-      const bool f16 = p.q.f16 != 0;
-      if (i < p.q.I) {
-        float b0 = 0.0f, b1 = 0.0f;
-        if (p.q.bias) {
-          b0 = from16(p.q.bias[i], f16);
-          if (FORM == FORM_GATED) b1 = from16(p.q.bias[p.q.I + i], f16);
-        }
-        // columns are dealt to the CTAs and to the two halves of their threads
-        for (int col = static_cast<int>(rank) * 2 + (threadIdx.x >> 7); col < left; col += 2 * p.split) {
-          float sum[2][1] = {{0.0f}, {0.0f}};
+    // A CTA finishes a run of the tile's columns, a thread four features of every eighth of them; what it adds is
+    // asked for before the wait.
+    const LinTile c = lin_tile(p, tstart, unit);
+    const bool f16 = p.q.f16 != 0;
+    const long long i = static_cast<long long>(c.ti) * p.feat + lane * 4;
+    const int left = static_cast<int>(min(p.q.J - static_cast<long long>(c.tj) * p.bn, static_cast<long long>(p.bn)));
+    const int share = (left + p.split - 1) / p.split;
+    const int end = min(left, (static_cast<int>(rank) + 1) * share);
+    int col = static_cast<int>(rank) * share + warp;
+    const long long row0 = static_cast<long long>(c.tj) * p.bn;
+    float b0[4] = {}, b1[4] = {};
+    uint16_t res[4] = {};
+    if (col < end) {
 #pragma unroll
-          for (int sub = 0; sub < SUBS; ++sub) {
-            const uint32_t at = smem_base + ((sub * p.bn + col) * 128 + f) * 4;
-            for (int r = 0; r < p.split; ++r) sum[sub][0] += ld_cluster_f32(map_to_cta(at, r));
+      for (int e = 0; e < 4; ++e)
+        if (i + e < p.q.I) {
+          if (p.q.bias) {
+            b0[e] = from16(p.q.bias[i + e], f16);
+            if (FORM == FORM_GATED) b1[e] = from16(p.q.bias[p.q.I + i + e], f16);
           }
-          lin_finish<1, FORM == FORM_GATED>(p.q, sum[0], sum[1], b0, b1, (j0 + col) * p.q.ldo + i, (j0 + col) * p.q.ldp + i, 1);
+          if (p.q.residual) res[e] = p.q.residual[(row0 + col) * p.q.ldo + i + e];
         }
+    }
+    cluster_sync_all();  // every CTA's partial sums are in its shared memory
+    for (; col < end; col += 8) {
+      float sum[2][4];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[sub][e] = 0.0f;
+        if (sub >= SUBS) continue;
+        const uint32_t at = smem_base + ((sub * p.bn + col) * 128 + lane * 4) * 4;
+        float4 got[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < p.split) got[r] = ld_cluster_f32x4(map_to_cta(at, r));
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < p.split) {
+            sum[sub][0] += got[r].x;
+            sum[sub][1] += got[r].y;
+            sum[sub][2] += got[r].z;
+            sum[sub][3] += got[r].w;
+          }
       }
+      uint16_t now[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        now[e] = res[e];
+        if (p.q.residual && col + 8 < end && i + e < p.q.I) res[e] = p.q.residual[(row0 + col + 8) * p.q.ldo + i + e];
+      }
+      lin_finish4<FORM == FORM_GATED>(p.q, sum[0], sum[1], b0, b1, now, i, row0 + col);
     }
   }
 
@@ -572,36 +728,97 @@ static size_t stage_size(const LinPick& c) {
   return (c.form == FORM_PLAIN ? 1 : 2) * static_cast<size_t>(kSubBytes) + static_cast<size_t>(c.bn / (c.pair ? 2 : 1)) * 128;
 }
 
-// Variant for a product, from its sizes.
-static LinPick pick_variant(const LinArgs& q, int sms) {
-  LinPick c;
-  memset(&c, 0, sizeof(c));
-  const int64_t groups = q.mode == LIN_ROWS ? q.groups : 1;
-  const int64_t avg = q.mode == LIN_ROWS ? ceil_div64(q.rows, groups < q.rows ? groups : q.rows) : q.J;
-  c.form = q.gated ? FORM_GATED : FORM_PLAIN;
-  c.split = 1;
-  const bool b_mn = q.b_mn != 0;
-  const int64_t many = q.mode == LIN_REDUCE ? q.groups : groups;
-  // pair tiles of 256 features x 256 tokens once they fill half of the GPU
-  const int64_t pair_tiles = many * ceil_div64(q.I, 256) * ceil_div64(avg, 256);
-  if (avg > 128 && pair_tiles * 2 * 2 >= sms) {
-    c.pair = true;
-    c.bn = 256;
-    if (!q.gated && many * ceil_div64(q.I, 512) * ceil_div64(avg, 256) * 2 >= sms) c.form = FORM_WIDE;
+// Time of a product under one variant, in SM cycles.  What the terms stand for, with what was measured:
+//   a stage costs its rows (128 bytes each) through the SM's port, 3.6 cycles a row, or its MMAs, the larger: bn / 2
+//   cycles of arithmetic per step of 16 and A sub-tile, but at least 137 per instruction of one issuing thread;
+//   rows fetched by number cost 45 cycles per four of them and loader warp;
+//   the epilogue issues about 12 instructions per result and warp, 16 more for an activation, 6 for a residual and for
+//   preact, half as many again in 2-byte accesses; it runs under the next tile's main loop where a second accumulator
+//   exists;
+//   a split reduction costs two cluster barriers and the exchange of its columns.
+static double variant_cycles(const LinArgs& q, const LinPick& c, int sms) {
+  const double blocks = q.mode == LIN_REDUCE ? static_cast<double>(q.rows) / q.groups / kKBlock + 0.5
+                                             : static_cast<double>(ceil_div64(q.K, kKBlock));
+  const int subs = c.form == FORM_PLAIN ? 1 : 2, mult = (c.pair ? 2 : 1) * (c.form == FORM_WIDE ? 2 : 1);
+  const double tiles_i = static_cast<double>(ceil_div64(q.I, 128 * mult));
+  double tiles;
+  if (q.mode == LIN_ROWS) {
+    // the rows of a group fill its tiles but for half of the last one
+    const double busy = static_cast<double>(q.groups < q.rows ? q.groups : q.rows);
+    tiles = static_cast<double>(q.rows) / c.bn + 0.5 * busy;
+    if (tiles < busy) tiles = busy;
   } else {
-    c.bn = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
-    if (b_mn && c.bn < 64) c.bn = 64;
-    if (q.mode == LIN_DENSE && c.bn <= 64) {
-      const int64_t tiles = ceil_div64(q.I, 128) * ceil_div64(q.J, c.bn), blocks = ceil_div64(q.K, kKBlock);
-      while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && blocks >= 4 * c.split * 2) c.split *= 2;
-    }
+    tiles = static_cast<double>(ceil_div64(q.J, c.bn)) * (q.mode == LIN_REDUCE ? q.groups : 1);
   }
-  return c;
+  tiles *= tiles_i * c.split;
+  const int per_sm = !c.pair && tiles > sms ? 2 : 1;
+  const double units = c.pair ? sms / 2 : sms * per_sm;
+  double waves = tiles / units;
+  if (q.mode != LIN_ROWS || waves < 1) waves = static_cast<double>(static_cast<int64_t>(waves + 0.999999));
+  else waves += 0.5;
+  const int bj = c.pair ? c.bn / 2 : c.bn;
+  double load = 3.6 * (128 * subs + bj) * per_sm;
+  if (q.mode == LIN_ROWS && q.gather_div && bj / 8 * 45.0 * 2 > load) load = bj / 8 * 45.0 * 2;
+  if (q.mode == LIN_REDUCE && q.gather_div) load += 8 * 2 * subs * 45.0;
+  const double math = 4.0 * subs * c.bn / 2 * per_sm;
+  const double stage = load > math ? (load > 548 ? load : 548) : (math > 548 ? math : 548);
+  const double main_loop = static_cast<double>(static_cast<int64_t>(blocks / c.split + 0.999999)) * stage;
+  double per_col = 12 + (q.act ? 16 : 0) + (q.residual ? 6 : 0) + (q.preact ? 6 * subs : 0) + (q.gated ? 4 : 0);
+  if (q.I % 8) per_col *= 1.5;
+  // warps of a scheduler take turns; a pair's eight warps share the columns, or each sub-tile's four take all of them
+  const double epi = c.pair ? per_col * (c.form == FORM_WIDE ? 2 * c.bn : c.bn) : per_col * c.bn * per_sm;
+  const bool covered = c.form == FORM_WIDE || c.form == FORM_PLAIN || (c.pair ? c.bn <= 128 : c.bn <= 64);
+  const double tile = covered ? (main_loop > epi ? main_loop : epi) : main_loop + epi;
+  double total = 3000 + (waves - 1) * tile + main_loop + epi;
+  if (c.split > 1) total += 3000 + 60.0 * c.bn / c.split;
+  return total;
+}
+
+// Variant for a product: the cheapest by the estimate above.
+static LinPick pick_variant(const LinArgs& q, int sms) {
+  LinPick best;
+  memset(&best, 0, sizeof(best));
+  double least = 1e300;
+  auto consider = [&](bool pair, int form, int bn, int split) {
+    LinPick c;
+    memset(&c, 0, sizeof(c));
+    c.pair = pair;
+    c.form = form;
+    c.bn = bn;
+    c.split = split;
+    const double t = variant_cycles(q, c, sms);
+    if (t < least) {
+      least = t;
+      best = c;
+    }
+  };
+  const int64_t most = q.mode == LIN_ROWS ? q.rows : q.J;  // no group has more tokens
+  const int step = q.b_mn ? 64 : 16;                       // an MN-major B is staged in blocks of 64
+  const int64_t blocks = ceil_div64(q.K, kKBlock);
+  for (int bn = step; bn <= 128; bn += bn < 64 ? step : 32) {
+    if (q.b_mn && bn % 64) continue;
+    const int form = q.gated ? FORM_GATED : FORM_PLAIN;
+    consider(false, form, bn, 1);
+    const int64_t tiles = ceil_div64(q.I, 128) * ceil_div64(q.J, bn);
+    if (q.mode == LIN_DENSE && bn <= 64)
+      for (int split = 2; split <= 8 && tiles * split <= 2 * sms && blocks >= 2 * split; split *= 2) consider(false, form, bn, split);
+    if (bn >= most) break;
+  }
+  if (most > 64 && sms >= 2)
+    for (int bn = 2 * step > 64 ? 2 * step : 64; bn <= 256; bn += q.b_mn ? 128 : 32) {
+      if (q.gated) {
+        consider(true, FORM_GATED, bn, 1);
+      } else {
+        consider(true, FORM_PLAIN, bn, 1);
+        consider(true, FORM_WIDE, bn, 1);
+      }
+      if (bn >= most) break;
+    }
+  return best;
 }
 
 template <bool PAIR, int FORM, int EPI, bool SPLIT>
-static int launch_variant(const CUtensorMap& a, const CUtensorMap& b, const LinUmma& p, int ctas, size_t smem,
-                          cudaStream_t stream) {
+static int launch_variant(const LinMaps& maps, const LinUmma& p, int ctas, size_t smem, cudaStream_t stream) {
   auto kern = linear_umma_kernel<PAIR, FORM, EPI, SPLIT>;
   static std::mutex mu;
   static bool done[64] = {false};
@@ -615,24 +832,8 @@ static int launch_variant(const CUtensorMap& a, const CUtensorMap& b, const LinU
       done[dev] = true;
     }
   }
-  cudaLaunchConfig_t lc;
-  memset(&lc, 0, sizeof(lc));
-  lc.gridDim = dim3(static_cast<unsigned>(ctas));
-  lc.blockDim = dim3(128 + 32 * EPI);
-  lc.dynamicSmemBytes = smem;
-  lc.stream = stream;
-  cudaLaunchAttribute attr[1];
-  if (PAIR || SPLIT) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = PAIR ? 2 : static_cast<unsigned>(p.split);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    lc.attrs = attr;
-    lc.numAttrs = 1;
-  }
-  const cudaError_t e = cudaLaunchKernelEx(&lc, kern, a, b, p);
-  count_launch();
-  return launch_status(e);
+  return launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), dim3(128 + 32 * EPI), smem, PAIR ? 2 : SPLIT ? p.split : 1,
+                           stream, maps, p);
 }
 
 int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cudaStream_t stream) {
@@ -647,9 +848,8 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
       if (pair != c.pair) c.form = q.gated ? FORM_GATED : FORM_PLAIN;
       c.pair = pair;
       if (cfg->tile_n) c.bn = cfg->tile_n;
-      if (pair && c.bn < 128) c.bn = 128;
+      if (pair && c.bn < 64) c.bn = 128;
       if (!pair && c.bn > 128) c.bn = 128;
-      if (c.form == FORM_WIDE && c.bn < 256) c.form = FORM_PLAIN;
       if (cfg->split_k) {
         c.split = cfg->split_k;
         if (c.split > 1 && c.bn > 64) c.bn = 64;
@@ -659,7 +859,8 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
     }
   }
   const bool two = !c.pair;
-  const size_t limit = (two ? kTwoCtas : kOneCta) - 1024;
+  const size_t turn = static_cast<size_t>(two ? 4 : 8) * kTurnFloats * sizeof(float);
+  const size_t limit = (two ? kTwoCtas : kOneCta) - 1024 - turn;
   int stages = static_cast<int>(limit / stage_size(c));
   if (stages > kLinStages) stages = kLinStages;
   if (cfg && cfg->stages) {
@@ -701,77 +902,66 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
   p.b_lbo = q.b_mn ? 8192 : 16;
   p.a_kadv = q.a_mn ? 2048 : 32;
   p.b_kadv = q.b_mn ? 2048 : 32;
+  const uintptr_t rows16 = reinterpret_cast<uintptr_t>(q.out) | reinterpret_cast<uintptr_t>(q.residual) | reinterpret_cast<uintptr_t>(q.preact);
+  p.vec = (rows16 & 15) == 0 && q.I % 8 == 0 && q.ldo % 8 == 0 && q.ldp % 8 == 0 && q.out_gs % 8 == 0;
   p.status = status ? status : fallback_status();
   if (!p.status) return FTB_E_CUDA;
 
   const CUtensorMapDataType dt = q.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint32_t ones[3] = {1, 1, 1};
-  CUtensorMap ma, mb;
-  int rc;
-  if (q.mode == LIN_REDUCE) {
-    // both operands are fetched row by row: 64 columns of four places per copy
-    const uint32_t box[2] = {64, 1};
-    const uint64_t da[2] = {static_cast<uint64_t>(q.I), static_cast<uint64_t>(q.gather_div ? q.src_rows : q.rows)};
-    const uint64_t db[2] = {static_cast<uint64_t>(q.J), static_cast<uint64_t>(q.rows)};
-    const uint64_t sa[1] = {static_cast<uint64_t>(q.lda) * 2}, sb[1] = {static_cast<uint64_t>(q.ldb) * 2};
-    rc = make_tmap(&ma, dt, 2, q.a, da, sa, box, ones);
-    if (!rc) rc = make_tmap(&mb, dt, 2, q.b, db, sb, box, ones);
-    if (rc) return rc;
-    p.oob_a = static_cast<int>(da[1]);
-    p.oob_b = static_cast<int>(db[1]);
-  } else {
-    const uint64_t a_rows = static_cast<uint64_t>(q.gated ? 2 * q.I : q.I);
-    const uint64_t a_groups = static_cast<uint64_t>(q.mode == LIN_ROWS ? q.groups : 1);
-    uint64_t d[3] = {static_cast<uint64_t>(q.K), a_rows, a_groups};
-    uint32_t box[3] = {64, 128, 1};
-    if (q.a_mn) {
-      d[0] = a_rows;
-      d[1] = static_cast<uint64_t>(q.K);
-      box[1] = 64;
+  LinMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  const bool reduce = q.mode == LIN_REDUCE, gathers = q.gather_div != 0;
+  int rc = FTB_OK;
+  {
+    // A: [group][row][k], or [group][k][i]; a reduction has one matrix of places
+    const uint64_t a_rows = static_cast<uint64_t>(q.gated ? 2 * q.I : q.I), kk = static_cast<uint64_t>(reduce ? q.rows : q.K);
+    const uint64_t d[3] = {q.a_mn ? a_rows : kk, q.a_mn ? kk : a_rows, static_cast<uint64_t>(q.mode == LIN_ROWS ? q.groups : 1)};
+    const uint32_t box[3] = {64, q.a_mn ? 64u : 128u, 1};
+    const uint64_t st[2] = {static_cast<uint64_t>(q.lda) * 2, d[1] * static_cast<uint64_t>(q.lda) * 2};
+    if (!(reduce && gathers)) rc = make_tmap(&maps.a, dt, 3, q.a, d, st, box, ones);
+    if (!rc && reduce) {
+      const uint64_t src = static_cast<uint64_t>(gathers ? q.src_rows : q.rows), dr[2] = {a_rows, src};
+      const uint32_t row_box[2] = {64, 1};
+      rc = make_tmap(&maps.a_rows, dt, 2, q.a, dr, st, row_box, ones);
+      p.oob_a = static_cast<int>(src);
     }
-    const uint64_t sa[2] = {static_cast<uint64_t>(q.lda) * 2, d[1] * static_cast<uint64_t>(q.lda) * 2};
-    rc = make_tmap(&ma, dt, 3, q.a, d, sa, box, ones);
     if (rc) return rc;
-    const uint64_t b_rows = static_cast<uint64_t>(q.mode == LIN_ROWS ? (q.gather_div ? q.src_rows : q.rows) : q.J);
-    if (q.gather_div) {
-      const uint64_t db[2] = {static_cast<uint64_t>(q.K), b_rows};
-      const uint64_t sb[1] = {static_cast<uint64_t>(q.ldb) * 2};
-      const uint32_t gbox[2] = {64, 1};
-      rc = make_tmap(&mb, dt, 2, q.b, db, sb, gbox, ones);
-      p.oob_b = static_cast<int>(b_rows);
-    } else {
-      uint64_t db[3] = {static_cast<uint64_t>(q.K), b_rows, 1};
-      uint32_t bbox[3] = {64, static_cast<uint32_t>(p.bj), 1};
-      if (q.b_mn) {
-        db[0] = b_rows;
-        db[1] = static_cast<uint64_t>(q.K);
-        bbox[1] = 64;
-      }
-      const uint64_t sb[2] = {static_cast<uint64_t>(q.ldb) * 2, db[1] * static_cast<uint64_t>(q.ldb) * 2};
-      rc = make_tmap(&mb, dt, 3, q.b, db, sb, bbox, ones);
+  }
+  {
+    const uint64_t rows = static_cast<uint64_t>(q.mode == LIN_ROWS ? (gathers ? q.src_rows : q.rows) : q.J);
+    const uint64_t kk = static_cast<uint64_t>(reduce ? q.rows : q.K);
+    const uint64_t d[3] = {q.b_mn ? rows : kk, q.b_mn ? kk : rows, 1};
+    const uint32_t box[3] = {64, q.b_mn ? 64u : static_cast<uint32_t>(p.bj), 1};
+    const uint64_t st[2] = {static_cast<uint64_t>(q.ldb) * 2, d[1] * static_cast<uint64_t>(q.ldb) * 2};
+    if (!(q.mode == LIN_ROWS && gathers)) rc = make_tmap(&maps.b, dt, 3, q.b, d, st, box, ones);
+    if (!rc && (reduce || (q.mode == LIN_ROWS && gathers))) {
+      const uint32_t row_box[2] = {64, 1};
+      rc = make_tmap(&maps.b_rows, dt, 2, q.b, d, st, row_box, ones);
+      p.oob_b = static_cast<int>(d[1]);
     }
     if (rc) return rc;
   }
 
-  size_t smem = static_cast<size_t>(stages) * stage_size(c) + 1024;
+  size_t smem = static_cast<size_t>(stages) * stage_size(c) + 1024 + turn;
   // A pair holds tensor memory while its CTAs wait for each other.  No other kernel with tensor memory may share the SM
   // with it (each could wait for columns that the other holds), so it always asks for most of the shared memory.
   if (c.pair && smem < 176 * 1024) smem = 176 * 1024;
   if (c.split > 1) {
     const int ctas = static_cast<int>(most) * c.split;
-    return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, true>(ma, mb, p, ctas, smem, stream)
-                                : launch_variant<false, FORM_PLAIN, 4, true>(ma, mb, p, ctas, smem, stream);
+    return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, true>(maps, p, ctas, smem, stream)
+                                : launch_variant<false, FORM_PLAIN, 4, true>(maps, p, ctas, smem, stream);
   }
   if (c.pair) {
     const int64_t units = sms / 2 < most ? sms / 2 : most;
     const int ctas = static_cast<int>(units) * 2;
-    if (c.form == FORM_GATED) return launch_variant<true, FORM_GATED, 8, false>(ma, mb, p, ctas, smem, stream);
-    if (c.form == FORM_WIDE) return launch_variant<true, FORM_WIDE, 8, false>(ma, mb, p, ctas, smem, stream);
-    return launch_variant<true, FORM_PLAIN, 8, false>(ma, mb, p, ctas, smem, stream);
+    if (c.form == FORM_GATED) return launch_variant<true, FORM_GATED, 8, false>(maps, p, ctas, smem, stream);
+    if (c.form == FORM_WIDE) return launch_variant<true, FORM_WIDE, 8, false>(maps, p, ctas, smem, stream);
+    return launch_variant<true, FORM_PLAIN, 8, false>(maps, p, ctas, smem, stream);
   }
   const int ctas = static_cast<int>(2 * sms < most ? 2 * sms : most);
-  return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, false>(ma, mb, p, ctas, smem, stream)
-                              : launch_variant<false, FORM_PLAIN, 4, false>(ma, mb, p, ctas, smem, stream);
+  return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, false>(maps, p, ctas, smem, stream)
+                              : launch_variant<false, FORM_PLAIN, 4, false>(maps, p, ctas, smem, stream);
 }
 
 }  // namespace ftb

@@ -1,6 +1,7 @@
 // What the feed-forward kernels share: 16-bit element conversion, the activations and their derivatives.
 #pragma once
 #include "ftb_host.h"
+#include "ftb_ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -48,6 +49,18 @@ constexpr float kGeluA = 0.044715f;
 // 1 / (1 + exp(-x)); exp overflows to infinity for very negative x, which gives the limit 0.
 __device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
+// Phi(z), the normal distribution function, and exp(-z^2/2) on the way: Abramowitz and Stegun 7.1.26 (erf to 1.5e-7),
+// one reciprocal and one exponential; the tail of a negative z is the product itself, without cancellation.
+__device__ __forceinline__ float normal_cdf(float z, float* bell) {
+  const float x = fabsf(z) * 0.7071067811865476f;
+  const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+  const float e = __expf(-x * x);
+  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float tail = 0.5f * poly * e;
+  *bell = e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
 // gelu_tanh(z) = z (1 + tanh(u)) / 2 = z sigmoid(2u).
 // __fdividef returns 0 for a denominator in (2^126, 2^128) and x / inf = 0, which is the limit here; only the product
 // with an infinite z needs care: relu keeps +inf, the others multiply z by a factor that has gone to 0 or 1, and
@@ -55,7 +68,10 @@ __device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, 1.
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case FTB_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-    case FTB_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    case FTB_ACT_GELU: {
+      float bell;
+      return z * normal_cdf(z, &bell);
+    }
     case FTB_ACT_GELU_TANH: return z * sigmoid_f(2.0f * kGeluC * (z + kGeluA * z * z * z));
     case FTB_ACT_SILU: return z * sigmoid_f(z);
     default: return z;
@@ -66,8 +82,11 @@ __device__ __forceinline__ float act_value(float z, int act) {
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case FTB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-    case FTB_ACT_GELU:
-      return 0.5f * (1.0f + erff(z * 0.7071067811865476f)) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    case FTB_ACT_GELU: {
+      float bell;
+      const float cdf = normal_cdf(z, &bell);
+      return fmaf(z * 0.3989422804014327f, bell, cdf);
+    }
     case FTB_ACT_GELU_TANH: {
       const float s = sigmoid_f(2.0f * kGeluC * (z + kGeluA * z * z * z));
       return s + 2.0f * z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
@@ -78,6 +97,77 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     }
     default: return 1.0f;
   }
+}
+
+// act(z) and act'(z) of N values: one branch, then straight-line code that shares the exponential.
+template <int N>
+__device__ __forceinline__ void act_both(const float (&z)[N], float (&value)[N], float (&slope)[N], int act) {
+  if (act == FTB_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float s = sigmoid_f(z[i]);
+      value[i] = z[i] * s;
+      slope[i] = s * (1.0f + z[i] * (1.0f - s));
+    }
+  } else if (act == FTB_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float bell;
+      const float cdf = normal_cdf(z[i], &bell);
+      value[i] = z[i] * cdf;
+      slope[i] = fmaf(z[i] * 0.3989422804014327f, bell, cdf);
+    }
+  } else if (act == FTB_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float q = z[i] * z[i], s = sigmoid_f(2.0f * kGeluC * z[i] * fmaf(kGeluA, q, 1.0f));
+      value[i] = z[i] * s;
+      slope[i] = fmaf(2.0f * z[i] * s * (1.0f - s) * kGeluC, fmaf(3.0f * kGeluA, q, 1.0f), s);
+    }
+  } else if (act == FTB_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      value[i] = z[i] < 0.0f ? 0.0f : z[i];
+      slope[i] = z[i] > 0.0f ? 1.0f : 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      value[i] = z[i];
+      slope[i] = 1.0f;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ launches that overlap
+// Every kernel of the feed-forward operators is launched as a programmatic dependent: its set-up runs while the kernel
+// before it in the stream drains.  Each waits (griddepcontrol.wait) before its first access to global memory, so what
+// an earlier kernel of any kind wrote is seen, and lets its own successor start only once it holds every resource that
+// it may have to wait for (tensor memory).
+template <typename... Params, typename... Args>
+inline int launch_overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream,
+                             Args... args) {
+  cudaLaunchConfig_t lc;
+  memset(&lc, 0, sizeof(lc));
+  lc.gridDim = grid;
+  lc.blockDim = block;
+  lc.dynamicSmemBytes = smem;
+  lc.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    lc.numAttrs = 2;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&lc, kernel, static_cast<Params>(args)...);
+  count_launch();
+  return launch_status(e);
 }
 
 }  // namespace ftb

@@ -293,10 +293,13 @@ __device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
-// A word of another CTA's shared memory (address from map_to_cta).
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// Four words of another CTA's shared memory (address from map_to_cta).
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 

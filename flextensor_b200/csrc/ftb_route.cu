@@ -6,6 +6,10 @@
 // experts.  Without bias and groups both scorings are monotone and the logits themselves are compared.  Otherwise
 // scores are computed in fp32 with a bound on their error; where two values that decide the result lie closer than
 // that bound, the warp computes the row's scores again in 64 bits and chooses by those.
+//
+// A lane's values become whole numbers in their order whose lowest bits are the value's place in the lane, and a
+// sorting network puts them in descending order once; every one of the top_k rounds then is a maximum over 32 heads and
+// a shift in the winning lane.  The bits given to the place widen the distance that counts as near.
 #include "ftb_lm.cuh"
 
 namespace ftb {
@@ -181,6 +185,8 @@ __device__ __forceinline__ float exp_below(float x, float m) { return m == -INFI
 
 template <int VPL>
 __device__ __noinline__ int choose_exactly(const RouteArgs& p, const float (&x)[VPL], uint32_t avail, float m, int lane) {
+  bool near = false;
+  if (!p.bias && p.groups == 1) return pick<float, VPL>(x, avail, p.top_k, -1.0f, lane, &near);
   double c[VPL];
   double sum = 0.0;
   const int e0 = lane * VPL;
@@ -198,13 +204,59 @@ __device__ __noinline__ int choose_exactly(const RouteArgs& p, const float (&x)[
     if (p.bias && ((avail >> v) & 1u)) c[v] += static_cast<double>(p.bias[e0 + v]);
     c[v] = c[v] != c[v] ? -INFINITY : c[v] + 0.0;
   }
-  bool near = false;
   if (p.groups > 1) avail = keep_groups<double, VPL>(p, c, avail, -1.0, lane, &near);
   return pick<double, VPL>(c, avail, p.top_k, -1.0, lane, &near);
 }
 
+// Batcher's odd-even merge sort of N keys in registers, largest first.
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int d = p; d > 0; d /= 2)
+#pragma unroll
+      for (int j = d % p; j + d < N; j += 2 * d)
+#pragma unroll
+        for (int i = 0; i < d; ++i)
+          if (i + j + d < N && (i + j) / (2 * p) == (i + j + d) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + d];
+            k[i + j] = max(a, b);
+            k[i + j + d] = min(a, b);
+          }
+}
+
+// pick() on sorted keys.  `tol` < 0: values that agree in every bit but the place's are near where `exact` is false.
+template <int VPL>
+__device__ __forceinline__ int pick_sorted(uint32_t (&k)[VPL], int count, float tol, bool exact, int lane, bool* near) {
+  constexpr uint32_t PLACE = VPL - 1;
+  int mine = 0;
+  uint32_t prev = 0;
+  for (int j = 0; j <= count; ++j) {
+    const uint32_t head = k[0] & ~PLACE, top = __reduce_max_sync(kAll, head);
+    if (top == 0) break;  // none left
+    if (j > 0) {
+      if (tol < 0.0f) *near |= !exact && prev == top;
+      else *near |= key_value(prev) - key_value(top) <= tol;
+    }
+    prev = top;
+    if (j == count) break;
+    const int winner = __ffs(__ballot_sync(kAll, head == top)) - 1;
+    const int id = __shfl_sync(kAll, lane * VPL + static_cast<int>(PLACE - (k[0] & PLACE)), winner);
+    if (lane == j) mine = id;
+    if (lane == winner) {
+#pragma unroll
+      for (int v = 0; v + 1 < VPL; ++v) k[v] = k[v + 1];
+      k[VPL - 1] = 0;
+    }
+  }
+  return mine;
+}
+
 template <typename T, int VPL>
 __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int lane = threadIdx.x & 31;
   const long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (t >= p.tokens) return;
@@ -224,10 +276,16 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
     for (int v = 0; v < VPL; ++v) m = fmaxf(m, x[v]);
     m = warp_max(m);
   }
+  constexpr uint32_t PLACE = VPL - 1;
+  uint32_t k[VPL];
+  bool near = false;
   int mine;
   if (by_logit) {
-    bool near = false;
-    mine = pick<float, VPL>(x, avail, p.top_k, -1.0f, lane, &near);
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) k[v] = ((avail >> v) & 1u) ? (order_key(x[v]) & ~PLACE) | (PLACE - v) : 0u;
+    sort_keys<VPL>(k);
+    // a 16-bit logit has no bits where the place goes
+    mine = pick_sorted<VPL>(k, p.top_k, -1.0f, sizeof(T) == 2 || VPL == 1, lane, &near);
     if (need_sum) {
 #pragma unroll
       for (int v = 0; v < VPL; ++v) total += exp_below(x[v], m);
@@ -238,30 +296,38 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
     float most = 0.0f;  // largest magnitude that enters a sum: what the error bound scales with
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      c[v] = sigmoid ? 1.0f / (1.0f + expf(-x[v])) : exp_below(x[v], m);
-      total += ((avail >> v) & 1u) ? c[v] : 0.0f;
+      c[v] = sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x[v])) : exp_below(x[v], m);
+      if (!sigmoid) total += ((avail >> v) & 1u) ? c[v] : 0.0f;
     }
-    total = warp_sum(total);
-    const float inv = sigmoid ? 1.0f : total > 0.0f ? 1.0f / total : 0.0f;
+    float inv = 1.0f;
+    if (!sigmoid) {
+      total = warp_sum(total);
+      inv = total > 0.0f ? 1.0f / total : 0.0f;
+    }
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      c[v] *= inv;
-      most = fmaxf(most, ((avail >> v) & 1u) ? c[v] : 0.0f);
-      if (p.bias && ((avail >> v) & 1u)) {
+      if (!sigmoid) c[v] *= inv;
+      const bool have_v = (avail >> v) & 1u;
+      if (have_v) most = fmaxf(most, c[v]);
+      if (p.bias && have_v) {
         const float b = p.bias[e0 + v];
         c[v] += b;
         if (fabsf(b) < INFINITY) most = fmaxf(most, fabsf(b));
       }
       c[v] = clean(c[v]);
     }
-    // exp and the reciprocals are good to a few units of 2^-24, the sum over the row to about 8 more
-    const float tol = 2e-6f * warp_max(most);
-    bool near = false;
+    // The exponentials and reciprocals are good to a few units of 2^-24 of the largest score (their error grows with
+    // |x|, where the score's slope has vanished faster), a sum over the row to about 8 more, and the place takes
+    // VPL units of a value of up to twice that.
+    const float tol = (3e-6f + VPL * 2.4e-7f) * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(most)));
     uint32_t left = avail;
     if (p.groups > 1) left = keep_groups<float, VPL>(p, c, avail, tol, lane, &near);
-    mine = pick<float, VPL>(c, left, p.top_k, tol, lane, &near);
-    if (near) mine = choose_exactly<VPL>(p, x, avail, m, lane);
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) k[v] = ((left >> v) & 1u) ? (order_key(c[v]) & ~PLACE) | (PLACE - v) : 0u;
+    sort_keys<VPL>(k);
+    mine = pick_sorted<VPL>(k, p.top_k, tol, false, lane, &near);
   }
+  if (near) mine = choose_exactly<VPL>(p, x, avail, m, lane);
 
   // weights: lane j < top_k has the j-th expert
   const bool active = lane < p.top_k;
@@ -299,6 +365,8 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
 // An expert that a row names twice gets both parts, added in the order of the slots.
 template <typename T, int VPL>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   __shared__ float grad[8][32 * VPL];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = static_cast<long long>(blockIdx.x) * 8 + warp;
@@ -383,21 +451,20 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) 
 }
 
 template <typename T, int VPL>
-static void launch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
-  const unsigned blocks = static_cast<unsigned>((p.tokens + 7) / 8);
-  if (backward) route_backward_kernel<T, VPL><<<blocks, 256, 0, stream>>>(p);
-  else route_kernel<T, VPL><<<blocks, 256, 0, stream>>>(p);
+static int launch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((p.tokens + 7) / 8));
+  return launch_overlapped(backward ? route_backward_kernel<T, VPL> : route_kernel<T, VPL>, grid, dim3(256), 0, 1, stream, p);
 }
 
 template <typename T>
-static void dispatch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
+static int dispatch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
   const int per = (p.experts + 31) / 32;
-  if (per <= 1) launch_route<T, 1>(p, backward, stream);
-  else if (per <= 2) launch_route<T, 2>(p, backward, stream);
-  else if (per <= 4) launch_route<T, 4>(p, backward, stream);
-  else if (per <= 8) launch_route<T, 8>(p, backward, stream);
-  else if (per <= 16) launch_route<T, 16>(p, backward, stream);
-  else launch_route<T, 32>(p, backward, stream);
+  if (per <= 1) return launch_route<T, 1>(p, backward, stream);
+  if (per <= 2) return launch_route<T, 2>(p, backward, stream);
+  if (per <= 4) return launch_route<T, 4>(p, backward, stream);
+  if (per <= 8) return launch_route<T, 8>(p, backward, stream);
+  if (per <= 16) return launch_route<T, 16>(p, backward, stream);
+  return launch_route<T, 32>(p, backward, stream);
 }
 
 static int route_checks(int dtype, int64_t tokens, int64_t experts, int64_t top_k, int scoring) {
@@ -414,11 +481,9 @@ static int run_route(int dtype, RouteArgs& p, bool backward, cudaStream_t stream
   const int esize = dtype == FTB_F32 ? 4 : 2;
   p.vec = (p.experts * esize) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 &&
           (!backward || (reinterpret_cast<uintptr_t>(p.dlogits) & 15) == 0);
-  if (dtype == FTB_F32) dispatch_route<float>(p, backward, stream);
-  else if (dtype == FTB_BF16) dispatch_route<__nv_bfloat16>(p, backward, stream);
-  else dispatch_route<__half>(p, backward, stream);
-  count_launch();
-  return launch_status(cudaSuccess);
+  if (dtype == FTB_F32) return dispatch_route<float>(p, backward, stream);
+  if (dtype == FTB_BF16) return dispatch_route<__nv_bfloat16>(p, backward, stream);
+  return dispatch_route<__half>(p, backward, stream);
 }
 
 }  // namespace ftb

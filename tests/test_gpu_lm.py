@@ -725,3 +725,156 @@ def test_expert_large(B, status, gather, gated):
         for name, got in (("dx", dx[a:c]), ("dw", dw[i]), ("db", db[i])):
             bounded(got, *want[name], "%s %d" % (name, i))
     assert not out[used:].any() and not dx[used:].any()
+
+
+# ---------------------------------------------------------------- together, as a model uses them
+class Block(object):
+    """A mixture-of-experts feed-forward block with a shared expert, forward and backward, on buffers of its own."""
+
+    def __init__(self, B, t=90, k=2, e=6, d=256, h=136, seed=0):
+        self.B, self.t, self.k, self.e, self.d, self.h = B, t, k, e, d, h
+        new = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, device="cuda", dtype=dtype)
+        self.x, self.dout = rand(seed, t, d), rand(seed + 1, t, d)
+        self.router = rand(seed + 2, 1, e, d, scale=d ** -0.5)
+        self.w1, self.w2 = rand(seed + 3, e, 2 * h, d, scale=d ** -0.5), rand(seed + 4, e, d, h, scale=h ** -0.5)
+        self.s1, self.s2 = rand(seed + 5, 2 * h, d, scale=d ** -0.5), rand(seed + 6, d, h, scale=h ** -0.5)
+        self.bias = rand(seed + 7, e, scale=0.05, dtype=torch.float32)
+        self.logits, self.ids, self.weights = new(1, t, e, dtype=torch.float32), new(t, k, dtype=torch.int32), new(t, k, dtype=torch.float32)
+        self.plan = B.ExpertPlan(t, k, e)
+        r = t * k
+        self.z1, self.a1, self.y = new(r, 2 * h), new(r, h), new(r, d)
+        self.zs, self.as_, self.shared, self.out = new(t, 2 * h), new(t, h), new(t, d), new(t, d)
+        self.dy, self.da, self.dz = new(r, d), new(r, h), new(r, d)
+        self.dw2, self.dw1, self.ds1, self.ds2 = new(e, d, h), new(e, 2 * h, d), new(2 * h, d), new(d, h)
+        self.dweights, self.dlogits, self.dx, self.das = new(t, k, dtype=torch.float32), new(t, e, dtype=torch.float32), new(t, d), new(t, h)
+        byte = lambda n: torch.empty(n, dtype=torch.uint8, device="cuda")
+        self.ws = byte(max(B.expert_linear_backward_workspace_bytes(self.plan, h, d, True),
+                           B.expert_linear_backward_workspace_bytes(self.plan, d, h),
+                           B.linear_backward_workspace_bytes(t, h, d, True), B.linear_backward_workspace_bytes(t, d, h)))
+        self.status = B.new_status()
+
+    def run(self):
+        B, st = self.B, self.status
+        B.bgemm_bf16(self.x[None], self.router, self.logits, trans_b=True, status=st)
+        logits = self.logits[0]
+        B.route_experts(logits, self.ids, self.weights, bias=self.bias, scoring="sigmoid")
+        B.expert_plan(self.ids, self.plan)
+        B.linear(self.x, self.s1, self.as_, activation="silu", gated=True, preact=self.zs, status=st)
+        B.linear(self.as_, self.s2, self.shared, residual=self.x, status=st)
+        B.expert_linear(self.x, self.w1, self.plan, self.a1, activation="silu", gated=True, gather=True, preact=self.z1, status=st)
+        B.expert_linear(self.a1, self.w2, self.plan, self.y, status=st)
+        B.expert_combine(self.y, self.plan, self.out, weights=self.weights, residual=self.shared)
+        B.expert_combine_backward(self.dout, self.plan, y=self.y, weights=self.weights, dy=self.dy, dweights=self.dweights)
+        B.expert_linear_backward(self.a1, self.w2, self.plan, self.dy, dx=self.da, dweight=self.dw2, workspace=self.ws, status=st)
+        B.expert_linear_backward(self.x, self.w1, self.plan, self.da, dx=self.dz, dweight=self.dw1, preact=self.z1, activation="silu",
+                                 gated=True, gather=True, workspace=self.ws, status=st)
+        B.expert_combine(self.dz, self.plan, self.dx)
+        B.route_experts_backward(logits, self.ids, self.dweights, self.dlogits, scoring="sigmoid")
+        B.linear_backward(self.as_, self.s2, self.dout, dx=self.das, dweight=self.ds2, workspace=self.ws, status=st)
+        B.linear_backward(self.x, self.s1, self.das, dweight=self.ds1, preact=self.zs, activation="silu", gated=True,
+                          workspace=self.ws, status=st)
+
+    def results(self):
+        return [self.out, self.weights, self.dw1, self.dw2, self.ds1, self.ds2, self.dx, self.dlogits]
+
+    def reference(self):
+        """The same by autograd in 64 bits, the choice of experts taken from the block."""
+        f = lambda v: v.double().requires_grad_(True)
+        x, w1, w2, s1, s2 = f(self.x), f(self.w1), f(self.w2), f(self.s1), f(self.s2)
+        logits = (self.x.double() @ self.router[0].double().T).requires_grad_(True)
+        ids = self.ids.long()
+        gate = lambda z: act64(z[:, : self.h], "silu") * z[:, self.h:]
+        w = torch.sigmoid(logits).gather(1, ids)
+        w = w / w.sum(1, keepdim=True)
+        parts = []
+        for e in range(self.e):
+            y = gate(x @ w1[e].T) @ w2[e].T
+            parts.append(y * (w * (ids == e)).sum(1, keepdim=True))
+        routed = sum(parts)
+        # the block's dx is that of the routed part alone
+        dx, = torch.autograd.grad((routed * self.dout.double()).sum(), x, retain_graph=True)
+        out = self.x.double() + gate(self.x.double() @ s1.T) @ s2.T + routed
+        g = torch.autograd.grad((out * self.dout.double()).sum(), [w1, w2, s1, s2, logits])
+        return [out, w, g[0], g[1], g[2], g[3], dx, g[4]]
+
+    def check(self):
+        self.B.check_status(self.status)
+        # a chain of four to five stores of 2^-8 each, relative to a result's own size (rms), eight times over
+        for got, want in zip(self.results(), self.reference()):
+            rms = float(want.square().mean().sqrt())
+            assert float((got.double() - want).abs().max()) <= 8 * 5 * 2.0 ** -8 * max(rms, float(want.abs().max()) / 8)
+            assert float((got.double() - want).square().mean().sqrt()) <= 5 * 2.0 ** -8 * rms
+
+
+def test_block(B):
+    block = Block(B)
+    block.run()
+    block.check()
+
+
+def test_block_long(B):
+    block = Block(B, t=1500, k=4, e=16, d=512, h=264, seed=20)
+    block.run()
+    block.check()
+
+
+def test_block_captured_and_replayed(B):
+    """One graph of the whole chain, replayed on new contents; a second graph of another block in between."""
+    first, second = Block(B), Block(B, t=33, seed=40)
+    want = []
+    graphs = []
+    for block in (first, second):
+        block.run()  # set-up outside the capture
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            block.run()
+        graphs.append(graph)
+    for seed in (60, 61):
+        first.x.copy_(rand(seed, first.t, first.d))
+        second.x.copy_(rand(seed + 5, second.t, second.d))
+        for v in first.results() + second.results():
+            v.zero_()
+        graphs[0].replay()
+        graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        first.check()
+        second.check()
+        kept = [v.clone() for v in first.results()]
+        first.run()
+        assert all(torch.equal(a, b) for a, b in zip(kept, first.results()))  # eager gives the same bits
+
+
+def test_block_on_another_stream(B):
+    """Two blocks at once on streams of their own, each behind work of its stream."""
+    blocks = [Block(B, seed=80), Block(B, t=64, k=3, seed=90)]
+    streams = [torch.cuda.Stream() for _ in blocks]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for block, stream in zip(blocks, streams):
+            with torch.cuda.stream(stream):
+                x = block.x.clone()
+                block.x.fill_(float("nan"))
+                torch.cuda._sleep(200000)
+                block.x.copy_(x)
+                block.run()
+    torch.cuda.synchronize()
+    for block in blocks:
+        block.check()
+
+
+def test_streams_are_named(B):
+    """The ``stream`` argument: the call runs behind that stream's work, not the current one's."""
+    x, w = rand(1, 64, 128), rand(2, 96, 128, scale=0.1)
+    want = torch.empty(64, 96, device="cuda", dtype=torch.bfloat16)
+    B.linear(x, w, want)
+    out, side = torch.empty_like(want), torch.cuda.Stream()
+    late = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(500000)
+        late.copy_(x)
+    B.linear(late, w, out, stream=side)
+    side.synchronize()
+    assert torch.equal(out, want)
