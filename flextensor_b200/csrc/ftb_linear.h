@@ -9,7 +9,7 @@ namespace ftb {
 // with features on i and tokens (or, for a weight's gradient, the weight's rows) on j.
 enum { LIN_DENSE = 0,   // one product
        LIN_ROWS = 1,    // j are sorted places, split by `offsets` into groups; A of group g
-       LIN_REDUCE = 2 }; // k are sorted places, split by `offsets`; one result per group
+       LIN_REDUCE = 2 }; // k are sorted places, split by `offsets`, of operands sorted already; one result per group
 
 struct LinArgs {
   int mode, f16;

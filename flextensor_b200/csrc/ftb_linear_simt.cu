@@ -36,8 +36,7 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinArgs p) {
           if (i < p.I && k < K) {
             const long long row = i + (s ? p.I : 0);
             if (p.mode == LIN_REDUCE) {
-              const long long r = gathered_row(p, lo + k);
-              if (r >= 0) v = from16(a[r * p.lda + row], f16);
+              v = from16(a[(lo + k) * p.lda + row], f16);
             } else {
               v = from16(p.a_mn ? a[k * p.lda + row] : a[row * p.lda + k], f16);
             }

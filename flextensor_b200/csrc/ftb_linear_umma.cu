@@ -13,8 +13,9 @@
 // Forms: FORM_PLAIN one A sub-tile; FORM_GATED two, the gate rows and the others of the same features, whose
 // accumulators share lanes and columns, so the gate is applied in registers; FORM_WIDE two neighbouring feature tiles
 // over the same tokens (a byte of B feeds twice the math).  PAIR runs two CTAs as one cta_group::2 unit.
-// SPLIT gives the reduction of one tile to the CTAs of a cluster, which add their fp32 partial sums through
-// distributed shared memory in rank order.
+// SPLIT gives the reduction of one tile to the CTAs of a cluster.  Every CTA finishes a run of the tile's columns; the
+// others write their fp32 partial sums of those into its shared memory, where they are added in rank order after one
+// cluster barrier (pulling them after the barrier instead cost 1.5 us more, and a second barrier before the exit).
 //
 // Waits are bounded as in ftb_umma_kernel.cuh: a role that gives up sets a status bit and the CTA leaves through its
 // normal teardown.
@@ -31,6 +32,26 @@ constexpr int kLinStages = 8;
 constexpr uint32_t kSubBytes = 128 * 128;  // 128 rows x 64 elements
 constexpr int kKBlock = 64;
 
+// Division by a number known on the host: the high word of a product with floor(2^32 / d) is at most one short.
+struct FastDiv {
+  uint32_t d, m;
+};
+static FastDiv fast_div(int64_t d) {
+  FastDiv f;
+  f.d = static_cast<uint32_t>(d);
+  f.m = d > 1 ? static_cast<uint32_t>((1ull << 32) / static_cast<uint64_t>(d)) : 0xffffffffu;
+  return f;
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t x, const FastDiv& f, uint32_t* rest) {
+  uint32_t q = __umulhi(x, f.m), r = x - q * f.d;
+  if (r >= f.d) {
+    ++q;
+    r -= f.d;
+  }
+  *rest = r;
+  return q;
+}
+
 struct LinUmma {
   LinArgs q;
   int bn, bj;            // tokens per tile, and of those staged per CTA
@@ -38,18 +59,21 @@ struct LinUmma {
   int tiles_i, tiles_j;  // tiles_j: LIN_DENSE and LIN_REDUCE
   int feat, sub_off;     // features per tile; feature rows between the A sub-tiles
   int band;              // token tiles walked together before the next feature tile
+  FastDiv by_i, by_group, by_span, by_band, by_last;  // tiles_i, tiles_i tiles_j, a band's tiles, its width, the last's
   int acc_slots;         // accumulators in turn (FORM_WIDE: one per sub-tile)
   uint32_t tmem_cols;
   uint32_t idesc;
   uint32_t a_lbo, b_lbo, a_kadv, b_kadv;
-  int oob_a, oob_b;      // a row past the gathered tensors
+  int oob_b;             // a row past the tensors whose rows are fetched by number
   int vec;               // rows of out, residual and preact start on 16 bytes
   int* status;
 };
 
 // Tiled maps of the operands, and maps whose boxes are one row high for rows fetched by number.
 struct LinMaps {
-  CUtensorMap a, b, a_rows, b_rows;
+  CUtensorMap a, b;            // a stage's boxes
+  CUtensorMap a_rows, b_rows;  // one row high, for rows fetched by number
+  CUtensorMap a16, b16;        // 16 k high, for the last block of a reduction
 };
 
 struct LinTile {
@@ -61,39 +85,41 @@ __device__ __forceinline__ LinTile lin_tile(const LinUmma& p, const int* tstart,
   c.g = 0;
   c.lo = 0;
   c.cnt = 0;
+  uint32_t r;
   if (p.q.mode == LIN_ROWS) {
-    // the group whose run of tiles holds t
+    // feature tiles run fastest; then the group whose token tiles hold this one
+    const int tok = static_cast<int>(div_by(t, p.by_i, &r));
+    c.ti = static_cast<int>(r);
     int a = 0, b = p.q.groups;
     while (b - a > 1) {
       const int mid = (a + b) >> 1;
-      if (static_cast<long long>(tstart[mid]) * p.tiles_i <= t) a = mid;
+      if (tstart[mid] <= tok) a = mid;
       else b = mid;
     }
     c.g = a;
-    const int nj = tstart[a + 1] - tstart[a], r = t - tstart[a] * p.tiles_i;
-    c.ti = r / nj;
-    c.tj = r - c.ti * nj;
+    c.tj = tok - tstart[a];
     int hi;
     group_range(p.q.offsets, a, p.q.rows, &c.lo, &hi);
     c.cnt = hi - c.lo;
     return c;
   }
-  const int per = p.tiles_i * p.tiles_j;
-  int r = t;
+  r = t;
   if (p.q.mode == LIN_REDUCE) {
-    c.g = t / per;
-    r = t - c.g * per;
+    c.g = static_cast<int>(div_by(t, p.by_group, &r));
     int hi;
     group_range(p.q.offsets, c.g, p.q.rows, &c.lo, &hi);
     c.cnt = hi - c.lo;
   }
   // bands of `band` token tiles: inside one, token tiles run fastest
-  const int span = p.band * p.tiles_i, b = r / span, first = b * p.band;
-  const int width = min(p.band, p.tiles_j - first), q = r - b * span;
-  c.ti = q / width;
-  c.tj = first + q - c.ti * width;
+  uint32_t q, x;
+  const int first = static_cast<int>(div_by(r, p.by_span, &q)) * p.band;
+  c.ti = static_cast<int>(first + p.band <= p.tiles_j ? div_by(q, p.by_band, &x) : div_by(q, p.by_last, &x));
+  c.tj = first + static_cast<int>(x);
   return c;
 }
+
+// Columns of a tile that one CTA of a split reduction finishes: a multiple of four.
+__host__ __device__ __forceinline__ int split_share(int columns, int split) { return ((columns + split - 1) / split + 3) & ~3; }
 
 __device__ __forceinline__ int lin_blocks(const LinUmma& p, const LinTile& c) {
   return p.q.mode == LIN_REDUCE ? (c.cnt + kKBlock - 1) / kKBlock : static_cast<int>((p.q.K + kKBlock - 1) / kKBlock);
@@ -135,43 +161,42 @@ struct WarpCols {
   int valid;          // columns that are tokens of this tile
 };
 
-// Reads the residual before the sums are ready: turned, 2 x 8 features; else 16 tokens of the lane's feature.
-__device__ __forceinline__ void lin_residual(const LinArgs& q, bool vec, const WarpCols& w, uint32_t (&res)[kCols],
-                                             const uint16_t* first) {
+// Reads the residual before the sums are ready: turned, 2 x 8 features; else 16 tokens of the lane's feature.  `r` is
+// the lane's own element of column 0.
+__device__ __forceinline__ void lin_residual(bool vec, const WarpCols& w, uint32_t (&res)[kCols], const uint16_t* r,
+                                             long long pitch) {
   if (vec) {
-    const uint16_t* r = first + (w.lane >> 2) * q.ldo + (w.lane & 3) * 8;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint4 x = make_uint4(0, 0, 0, 0);
-      if (w.live8 && (w.lane >> 2) + 8 * h < w.valid) x = *reinterpret_cast<const uint4*>(r + 8 * h * q.ldo);
+      if (w.live8 && (w.lane >> 2) + 8 * h < w.valid) x = *reinterpret_cast<const uint4*>(r + (h ? 8 * pitch : 0));
       res[4 * h] = x.x;
       res[4 * h + 1] = x.y;
       res[4 * h + 2] = x.z;
       res[4 * h + 3] = x.w;
     }
   } else {
-    const uint16_t* r = first + w.lane;
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       res[c] = w.live && c < w.valid ? *r : 0u;
-      r += q.ldo;
+      r += pitch;
     }
   }
 }
 
-// Rounds and stores the warp's 16 x 32 values; `first` is the element of column 0 and lane 0, `res` null or the residual.
-__device__ __forceinline__ void lin_store(bool vec, bool f16, const WarpCols& w, float (&v)[kCols], uint16_t* first,
+// Rounds and stores the warp's 16 x 32 values; `o` is the lane's own element of column 0, `res` null or the residual.
+__device__ __forceinline__ void lin_store(bool vec, bool f16, const WarpCols& w, float (&v)[kCols], uint16_t* o,
                                           long long pitch, const uint32_t* res) {
   if (vec) {
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < kCols; ++c) w.turn[c * kTurnPitch + w.lane] = v[c];
     __syncwarp();
-    const int tok = w.lane >> 2, oct = (w.lane & 3) * 8;
+    const int tok = w.lane >> 2;
+    const float4* from = reinterpret_cast<const float4*>(w.turn + tok * kTurnPitch + (w.lane & 3) * 8);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4 a = *reinterpret_cast<const float4*>(w.turn + (tok + 8 * h) * kTurnPitch + oct);
-      const float4 b = *reinterpret_cast<const float4*>(w.turn + (tok + 8 * h) * kTurnPitch + oct + 4);
+      const float4 a = from[h * 8 * kTurnPitch / 4], b = from[h * 8 * kTurnPitch / 4 + 1];
       float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
       if (res) {
 #pragma unroll
@@ -182,11 +207,10 @@ __device__ __forceinline__ void lin_store(bool vec, bool f16, const WarpCols& w,
         }
       }
       if (w.live8 && tok + 8 * h < w.valid)
-        *reinterpret_cast<uint4*>(first + (tok + 8 * h) * pitch + oct) =
+        *reinterpret_cast<uint4*>(o + (h ? 8 * pitch : 0)) =
             make_uint4(pack16(x[0], x[1], f16), pack16(x[2], x[3], f16), pack16(x[4], x[5], f16), pack16(x[6], x[7], f16));
     }
   } else {
-    uint16_t* o = first + w.lane;
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       float x = v[c];
@@ -197,21 +221,29 @@ __device__ __forceinline__ void lin_store(bool vec, bool f16, const WarpCols& w,
   }
 }
 
-template <bool GATED>
+// RICH = false: nothing but the store.  (In one kernel with the rest, the jumps over its code cost a short reduction
+// as much as the store itself: 600 cycles per 16 columns and warp.)
+template <bool GATED, bool RICH>
 __device__ __forceinline__ void lin_finish(const LinArgs& q, bool vec, const WarpCols& w, float (&v)[kCols],
                                            float (&u)[kCols], const uint32_t (&res)[kCols], float b0, float b1,
                                            uint16_t* out, uint16_t* preact) {
   const bool f16 = q.f16 != 0;
+  if constexpr (!RICH) {
+    lin_store(vec, f16, w, v, out, q.ldo, nullptr);
+    return;
+  }
+  if (q.bias) {
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    v[c] += b0;
-    if constexpr (GATED) u[c] += b1;
+    for (int c = 0; c < kCols; ++c) {
+      v[c] += b0;
+      if constexpr (GATED) u[c] += b1;
+    }
   }
   if (q.preact) {
     lin_store(vec, f16, w, v, preact, q.ldp, nullptr);
     if constexpr (GATED) lin_store(vec, f16, w, u, preact + q.I, q.ldp, nullptr);
   }
-  act_values<kCols>(v, q.act);
+  if (q.act) act_values<kCols>(v, q.act);
   if constexpr (GATED) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c) v[c] *= u[c];
@@ -219,41 +251,36 @@ __device__ __forceinline__ void lin_finish(const LinArgs& q, bool vec, const War
   lin_store(vec, f16, w, v, out, q.ldo, q.residual ? res : nullptr);
 }
 
-// The same for four neighbouring features of one token (after a split reduction).
+// The same for four tokens of one feature (after a split reduction).
 template <bool GATED>
-__device__ __forceinline__ void lin_finish4(const LinArgs& q, float (&v)[4], float (&u)[4], const float (&b0)[4],
-                                            const float (&b1)[4], const uint16_t (&res)[4], long long i, long long row) {
+__device__ __forceinline__ void lin_finish4(const LinArgs& q, float (&v)[4], float (&u)[4], float b0, float b1,
+                                            const uint16_t (&res)[4], long long i, long long row, int valid) {
   const bool f16 = q.f16 != 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    v[e] += b0[e];
-    if constexpr (GATED) u[e] += b1[e];
+    v[e] += b0;
+    if constexpr (GATED) u[e] += b1;
   }
   if (q.preact) {
+    uint16_t* z = q.preact + row * q.ldp + i;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (i + e < q.I) {
-        q.preact[row * q.ldp + i + e] = to16(v[e], f16);
-        if constexpr (GATED) q.preact[row * q.ldp + q.I + i + e] = to16(u[e], f16);
+      if (e < valid) {
+        z[e * q.ldp] = to16(v[e], f16);
+        if constexpr (GATED) z[e * q.ldp + q.I] = to16(u[e], f16);
       }
   }
   act_values<4>(v, q.act);
+  uint16_t* out = q.out + row * q.ldo + i;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if constexpr (GATED) v[e] *= u[e];
     if (q.residual) v[e] += from16(res[e], f16);
-  }
-  uint16_t* out = q.out + row * q.ldo + i;
-  if (i + 3 < q.I && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack16(v[0], v[1], f16), pack16(v[2], v[3], f16));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < q.I) out[e] = to16(v[e], f16);
+    if (e < valid) out[e * q.ldo] = to16(v[e], f16);
   }
 }
 
-template <bool PAIR, int FORM, int EPI, bool SPLIT>
+template <bool PAIR, int FORM, int EPI, bool SPLIT, bool RICH>
 __global__ void __launch_bounds__(128 + 32 * EPI, EPI == 4 ? 2 : 1)
 linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinUmma p) {
   extern __shared__ uint8_t smem_raw[];
@@ -268,7 +295,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   constexpr int SUBS = FORM == FORM_PLAIN ? 1 : 2;
   static_assert(!SPLIT || (!PAIR && FORM != FORM_WIDE && EPI == 4), "the reduction is split in single-CTA tiles only");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t b_bytes = static_cast<uint32_t>(p.bj) * 128u;
   const uint32_t stage_bytes = SUBS * kSubBytes + b_bytes;
@@ -278,6 +305,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   const uint32_t stages = p.stages;
   const int mode = p.q.mode;
 
+  if constexpr (SPLIT) cluster_arrive();  // this CTA runs: its shared memory can be written from now on
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < stages; ++s) {
@@ -328,7 +356,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();  // the peer's barriers exist before anything signals them
   tc_fence_after();
-  const uint32_t tmem_base = tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_slot, 0);
   grid_launch_dependents();  // tensor memory is held: a successor's CTA on this SM cannot take it first
   grid_dependency_wait();
 
@@ -337,8 +365,8 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   const uint32_t tfull0 = smem_u32(&bar_tfull[0]), tempty0 = smem_u32(&bar_tempty[0]);
   const uint32_t slot_stride = FORM == FORM_WIDE ? static_cast<uint32_t>(p.bn) : static_cast<uint32_t>(p.bn) * SUBS;
 
-  // Rows by number: tokens of a group (gather_j), or places of a reduction whose operand is not sorted or whose last
-  // block ends inside it (gather_k).  One thread gets a gather4 out about every 25 ns, so two warps share them.
+  // Rows by number: tokens of a group (gather_j), or the places of a reduction's last block (gather_k), of which those
+  // past the group are asked for outside the tensors.  Two warps share the copies.
   const bool gather_j = mode == LIN_ROWS && p.q.gather_div != 0;
   const bool gather_k = mode == LIN_REDUCE;
   if (warp == 0 || (warp == 3 && (gather_j || gather_k))) {
@@ -373,39 +401,25 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
       }
       for (int kb = kb0; kb < kb1; ++kb) {
         const bool tail = gather_k && (kb + 1) * kKBlock > c.cnt;   // the block ends past the group
-        const bool rows_a = gather_k && (tail || p.q.gather_div != 0), rows_b = tail;
-        if (rows_a) {
-          // quads 0..7: this warp's half of the block's places in A, 8..15: in B
-          __syncwarp();
-          if (lane < 16) {
-            int row[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int k = kb * kKBlock + (part * 8 + (lane & 7)) * 4 + e;
-              if (lane < 8) {
-                const long long r = k < c.cnt ? gathered_row(p.q, c.lo + k) : -1;
-                row[e] = r >= 0 ? static_cast<int>(r) : p.oob_a;
-              } else {
-                row[e] = k < c.cnt ? c.lo + k : p.oob_b;
-              }
-            }
-            quads[lane] = make_int4(row[0], row[1], row[2], row[3]);
-          }
-          __syncwarp();
-        }
-        if (lane == 0) {
-          ok = mbar_wait(empty0 + 8 * s, ph ^ 1u, &abort_flag);
-          if (!ok) {
+        
+        // The last block of a group: whole runs of 16 places as tiles (an MMA takes 16), the places of the run in which
+        // the group ends by number, those past it outside the tensors.
+        const int runs = tail ? (c.cnt - kb * kKBlock) >> 4 : 0, odd = tail ? (c.cnt - kb * kKBlock) & 15 : 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ph ^ 1u, &abort_flag));
+        if (!ok) {
+          if (lane == 0) {
             atomicOr(p.status, FTB_DEV_WAIT_EMPTY);
             abort_flag = 1;
           }
+          break;
         }
-        if (lane == 0 && ok) {
+        if (elect_one()) {
           const uint32_t full = sig0 + 8 * s, sb = sa + SUBS * kSubBytes;
           const int kc = gather_k ? c.lo + kb * kKBlock : kb * kKBlock;
           if (part == 0) {
-            if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR ? 2 * tx : tx);
-            if (!rows_a) {
+            const uint32_t bytes = tail ? tx / 4 * (runs + (odd ? 1 : 0)) : tx;
+            if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR ? 2 * bytes : bytes);
+            if (!tail) {
 #pragma unroll
               for (int sub = 0; sub < SUBS; ++sub) {
                 const uint32_t dst = sa + sub * kSubBytes;
@@ -423,7 +437,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
               }
             }
             if (p.q.b_mn) {
-              if (!rows_b) {
+              if (!tail) {
                 for (int b = 0; b * 64 < p.bj; ++b) {
                   if constexpr (PAIR) tma_load_3d_pair(sb + b * 8192u, &maps.b, full, j0 + b * 64, kc, 0);
                   else tma_load_3d(sb + b * 8192u, &maps.b, full, j0 + b * 64, kc, 0);
@@ -443,29 +457,31 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
               else tma_gather4(dst, &maps.b_rows, full, kc, r.x, r.y, r.z, r.w);
             }
           }
-          if (rows_a) {
-            for (int e = 0; e < 8; ++e) {
-              const int4 r = quads[e];
-              const uint32_t at = static_cast<uint32_t>(part * 8 + e) * 512u;
-#pragma unroll
-              for (int b = 0; b < 2 * SUBS; ++b) {
-                const uint32_t dst = sa + b * 8192u + at;
-                const int col = f0 + (b >> 1) * p.sub_off + (b & 1) * 64;
-                if constexpr (PAIR) tma_gather4_pair(dst, &maps.a_rows, full, col, r.x, r.y, r.z, r.w);
-                else tma_gather4(dst, &maps.a_rows, full, col, r.x, r.y, r.z, r.w);
+          if (tail) {
+            for (int x = 0; x < 2 * SUBS + (p.bj >> 6); ++x) {
+              const bool in_a = x < 2 * SUBS;
+              const int y = x - 2 * SUBS;
+              const uint32_t dst = in_a ? sa + x * 8192u : sb + y * 8192u;
+              const int col = in_a ? f0 + (x >> 1) * p.sub_off + (x & 1) * 64 : j0 + y * 64;
+              if ((x & 1) != part) continue;  // the two loader warps take turns
+              const CUtensorMap* m16 = in_a ? &maps.a16 : &maps.b16;
+              const CUtensorMap* m1 = in_a ? &maps.a_rows : &maps.b_rows;
+              for (int r = 0; r < runs; ++r) {
+                if constexpr (PAIR) tma_load_3d_pair(dst + r * 2048u, m16, full, col, kc + r * 16, 0);
+                else tma_load_3d(dst + r * 2048u, m16, full, col, kc + r * 16, 0);
               }
-              if (rows_b) {
-                const int4 q = quads[8 + e];
-                for (int b = 0; b * 64 < p.bj; ++b) {
-                  if constexpr (PAIR) tma_gather4_pair(sb + b * 8192u + at, &maps.b_rows, full, j0 + b * 64, q.x, q.y, q.z, q.w);
-                  else tma_gather4(sb + b * 8192u + at, &maps.b_rows, full, j0 + b * 64, q.x, q.y, q.z, q.w);
-                }
+              for (int e = 0; odd && e < 4; ++e) {
+                const int k = e * 4, base = kc + runs * 16;
+                const int r0 = k < odd ? base + k : p.oob_b, r1 = k + 1 < odd ? base + k + 1 : p.oob_b;
+                const int r2 = k + 2 < odd ? base + k + 2 : p.oob_b, r3 = k + 3 < odd ? base + k + 3 : p.oob_b;
+                const uint32_t at = dst + runs * 2048u + e * 512u;
+                if constexpr (PAIR) tma_gather4_pair(at, m1, full, col, r0, r1, r2, r3);
+                else tma_gather4(at, m1, full, col, r0, r1, r2, r3);
               }
             }
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok) break;
+        __syncwarp();
         sa += stage_bytes;
         if (++s == stages) {
           s = 0;
@@ -478,13 +494,14 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   } else if (warp == 1 || (SUBS == 2 && warp == 2)) {
     // ------------------------------------------------------------ MMA issuers (leader CTA of a pair)
     const uint32_t sub = warp - 1;
-    if (lane == 0 && (!PAIR || rank == 0)) {
+    if (!PAIR || rank == 0) {
       const uint32_t idesc = p.idesc;
       const uint32_t a_hi = smem_desc_hi(p.a_lbo, 1024, 2), b_hi = smem_desc_hi(p.b_lbo, 1024, 2);
       const uint32_t a_lo0 = smem_desc_lo(smem_base + sub * kSubBytes, p.a_lbo);
       const uint32_t b_lo0 = smem_desc_lo(smem_base + SUBS * kSubBytes, p.b_lbo);
       const uint32_t a_k = p.a_kadv >> 4, b_k = p.b_kadv >> 4, stage_enc = stage_bytes >> 4;
-      uint32_t s = 0, ph = 0, off = 0, ready = 0;
+      uint32_t s = 0, ph = 0, off = 0;
+      bool ready = false;
       int local = 0;
       bool ok = true;
       for (int t = unit; t < total && ok; t += units, ++local) {
@@ -494,34 +511,43 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
         const int kb0 = SPLIT ? static_cast<int>(rank) * per : 0, kb1 = min(blocks, kb0 + per);
         const uint32_t acc = FORM == FORM_WIDE ? sub : p.acc_slots == 2 ? local & 1u : 0u;
         const uint32_t aph = FORM != FORM_WIDE && p.acc_slots == 2 ? (local >> 1) & 1u : local & 1u;
-        if (!mbar_wait(tempty0 + 8 * acc, aph ^ 1u, &abort_flag)) {
-          atomicOr(p.status, FTB_DEV_WAIT_TMEMFREE);
-          abort_flag = 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(tempty0 + 8 * acc, aph ^ 1u, &abort_flag))) {
+          if (lane == 0) {
+            atomicOr(p.status, FTB_DEV_WAIT_TMEMFREE);
+            abort_flag = 1;
+          }
           break;
         }
         tc_fence_after();
         const uint32_t d = tmem_base + acc * slot_stride + (FORM == FORM_GATED ? sub * static_cast<uint32_t>(p.bn) : 0u);
         uint32_t accumulate = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!ready && !mbar_wait(full0 + 8 * s, ph, &abort_flag)) {
-            atomicOr(p.status, FTB_DEV_WAIT_FULL);
-            abort_flag = 1;
+          if (!ready && !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, ph, &abort_flag))) {
+            if (lane == 0) {
+              atomicOr(p.status, FTB_DEV_WAIT_FULL);
+              abort_flag = 1;
+            }
             ok = false;
             break;
           }
           tc_fence_after();
-          {
-            // has the next stage landed?  (the answer is used in the next iteration)
-            const uint32_t sn = s + 1 == stages ? 0u : s + 1;
-            ready = mbar_test_wait(full0 + 8 * sn, sn == 0 ? ph ^ 1u : ph);
-          }
           const uint32_t a_lo = a_lo0 + off, b_lo = b_lo0 + off;
+          // steps of 16 that hold something: the last block of a reduction may have fewer than four
+          const int steps = gather_k ? min(4, (c.cnt - kb * kKBlock + 15) >> 4) : 4;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma<KIND_BF16, PAIR>(d, a_lo + k * a_k, a_hi, b_lo + k * b_k, b_hi, idesc, k > 0 ? 1u : accumulate);
+            for (int k = 0; k < 4; ++k)
+              if (k < steps) umma<KIND_BF16, PAIR>(d, a_lo + k * a_k, a_hi, b_lo + k * b_k, b_hi, idesc, k > 0 ? 1u : accumulate);
+            if constexpr (PAIR) tc_commit_pair_both(empty0 + 8 * s);
+            else tc_commit(empty0 + 8 * s);
+          }
+          __syncwarp();
+          {
+            // has the next stage landed?
+            const uint32_t sn = s + 1 == stages ? 0u : s + 1;
+            ready = __all_sync(0xffffffffu, mbar_test_wait(full0 + 8 * sn, sn == 0 ? ph ^ 1u : ph));
+          }
           accumulate = 1;
-          if constexpr (PAIR) tc_commit_pair_both(empty0 + 8 * s);
-          else tc_commit(empty0 + 8 * s);
           off += stage_enc;
           if (++s == stages) {
             s = 0;
@@ -529,10 +555,11 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
             off = 0;
           }
         }
-        if (ok) {
+        if (ok && elect_one()) {
           if constexpr (PAIR) tc_commit_pair_both(tfull0 + 8 * acc);
           else tc_commit(tfull0 + 8 * acc);
         }
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -542,6 +569,8 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
     constexpr int GROUPS = EPI / 4;
     const uint32_t tempty_sig = PAIR ? map_to_cta(tempty0, 0) : tempty0;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const long long lane_ldo = p.vec ? (lane >> 2) * p.q.ldo + (lane & 3) * 8 : lane;
+    const long long lane_ldp = p.vec ? (lane >> 2) * p.q.ldp + (lane & 3) * 8 : lane;
     int local = 0;
     for (int t = unit; t < total; t += units, ++local) {
       const LinTile c = lin_tile(p, tstart, t);
@@ -553,7 +582,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
                           (PAIR ? rank * 128 : 0) + quarter * 32 + lane;
       const bool live = i < p.q.I;
       float b0 = 0.0f, b1 = 0.0f;
-      if (!SPLIT && live && p.q.bias) {
+      if (!SPLIT && RICH && live && p.q.bias) {
         const uint16_t* bias = p.q.bias + c.g * p.q.bias_gs + i;
         b0 = from16(bias[0], p.q.f16 != 0);
         if (FORM == FORM_GATED) b1 = from16(bias[p.q.I], p.q.f16 != 0);
@@ -565,62 +594,89 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
       const long long out_base = mode == LIN_REDUCE ? c.g * p.q.out_gs : 0;
       constexpr bool GATED = FORM == FORM_GATED;
       const int first = FORM == FORM_WIDE ? 0 : grp * kCols, step = FORM == FORM_WIDE ? kCols : GROUPS * kCols;
-      const bool vec = p.vec != 0, add = !SPLIT && p.q.residual != nullptr;
+      const bool vec = p.vec != 0, add = !SPLIT && RICH && p.q.residual != nullptr;
       WarpCols w;
       w.turn = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)) + stages * stage_bytes) + (warp - 4) * kTurnFloats;
       w.lane = lane;
       w.live = live;
       w.live8 = i - lane + (lane & 3) * 8 < p.q.I;
-      const long long i0 = i - lane;  // the warp's first feature
+      // this lane's element of the warp's first column in out and residual, and in preact
+      long long at = out_base + (row0 + first) * p.q.ldo + (i - lane) + lane_ldo;
+      long long zat = (row0 + first) * p.q.ldp + (i - lane) + lane_ldp;
+      const long long at_step = step * p.q.ldo, zat_step = step * p.q.ldp;
       uint32_t res[kCols];
       w.valid = left - first;
-      if (add) lin_residual(p.q, vec, w, res, p.q.residual + out_base + (row0 + first) * p.q.ldo + i0);
+      if (add) lin_residual(vec, w, res, p.q.residual + at, p.q.ldo);
       const bool got = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, aph, &abort_flag));
       if (!got) {
         if (lane == 0) {
           atomicOr(p.status, FTB_DEV_WAIT_TMEMFULL);
           abort_flag = 1;
         }
+        if constexpr (SPLIT) {  // the barriers that the other warps and CTAs wait at
+          cluster_wait();
+          named_barrier_arrive(1, 160);
+        }
         break;
       }
       tc_fence_after();
       const uint32_t d = tmem_base + lanes + acc * slot_stride;
       if constexpr (SPLIT) {
-        // fp32 partial sums into the (now idle) stages, [sub][column][lane]
-        float* part = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));
+        // fp32 partial sums to the CTAs that finish their columns: [source rank][sub][four columns][feature][column]
         const int per = (lin_blocks(p, c) + p.split - 1) / p.split;
         const bool mine = static_cast<int>(rank) * per < lin_blocks(p, c);
+        const int share = split_share(left, p.split);
+        const uint32_t inbox = smem_base + stages * stage_bytes;
+        cluster_wait();  // every CTA of the cluster has started
         for (int sub = 0; sub < SUBS; ++sub)
           for (int c0 = 0; c0 < p.bn && c0 < left; c0 += 16) {
             uint32_t v[16];
             tmem_ld_32x16(d + sub * p.bn + c0, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (c0 + e < left) part[(sub * p.bn + c0 + e) * 128 + quarter * 32 + lane] = mine ? __uint_as_float(v[e]) : 0.0f;
+            for (int e = 0; e < 16; e += 4)
+              if (c0 + e < left) {
+                const int owner = (c0 + e) / share, quad = ((c0 + e) - owner * share) >> 2;
+                const uint32_t to = inbox + ((((rank * SUBS + sub) * (share >> 2) + quad) * 128 + quarter * 32 + lane) << 4);
+                st_cluster_f32x4(map_to_cta(to, owner), mine ? __uint_as_float(v[e]) : 0.0f, mine ? __uint_as_float(v[e + 1]) : 0.0f,
+                                 mine ? __uint_as_float(v[e + 2]) : 0.0f, mine ? __uint_as_float(v[e + 3]) : 0.0f);
+              }
           }
+        tc_fence_before();
+        named_barrier_arrive(1, 160);  // tensor memory has been read
         break;  // one tile per cluster
       } else {
-        for (int c0 = first; c0 < p.bn && c0 < left; c0 += step) {
-          uint32_t rv[kCols], ru[kCols], now[kCols];
+        uint32_t rv[kCols], ru[kCols];
+        auto load = [&](int at) {
+          tmem_ld_32x16(d + at, rv);
+          if constexpr (GATED) tmem_ld_32x16(d + p.bn + at, ru);
+        };
+        const int stop = min(p.bn, left);
+        if (first < stop) load(first);
+        for (int c0 = first; c0 < stop; c0 += step) {
+          uint32_t now[kCols];
           float v[kCols], u[kCols];
-          tmem_ld_32x16(d + c0, rv);
-          if constexpr (GATED) tmem_ld_32x16(d + p.bn + c0, ru);
 #pragma unroll
           for (int e = 0; e < kCols; ++e) now[e] = res[e];
           if (add && c0 + step < left) {
             w.valid = left - c0 - step;
-            lin_residual(p.q, vec, w, res, p.q.residual + out_base + (row0 + c0 + step) * p.q.ldo + i0);
+            lin_residual(vec, w, res, p.q.residual + at + at_step, p.q.ldo);
           }
           w.valid = left - c0;
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < kCols; ++e) {
-            v[e] = work ? __uint_as_float(rv[e]) : 0.0f;
+            v[e] = __uint_as_float(rv[e]);
             if constexpr (GATED) u[e] = __uint_as_float(ru[e]);
           }
-          lin_finish<GATED>(p.q, vec, w, v, u, now, b0, b1, p.q.out + out_base + (row0 + c0) * p.q.ldo + i0,
-                            p.q.preact + (row0 + c0) * p.q.ldp + i0);
+          if (!work) {
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) v[e] = 0.0f;
+          }
+          if (c0 + step < stop) load(c0 + step);
+          lin_finish<GATED, RICH>(p.q, vec, w, v, u, now, b0, b1, p.q.out + at, p.q.preact + zat);
+          at += at_step;
+          zat += zat_step;
         }
         tc_fence_before();
         __syncwarp();
@@ -636,65 +692,58 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   if constexpr (SPLIT) {
     // Tensor memory goes back before this CTA waits for its peers: a CTA of another kernel that waits for columns of
     // this SM then never holds up a peer that this cluster waits for.
-    tc_fence_before();
-    __syncthreads();
     if (warp == 1) {
+      named_barrier_sync(1, 160);
       tc_fence_after();
       tmem_dealloc(tmem_base, p.tmem_cols);
     }
+    if (warp < 4) cluster_wait();  // (the epilogue has waited for the start already)
     __syncwarp();
-    // A CTA finishes a run of the tile's columns, a thread four features of every eighth of them; what it adds is
-    // asked for before the wait.
+    cluster_arrive();
+    // A CTA finishes a run of the tile's columns, a thread four of one feature at a time; what it adds is asked for
+    // before the wait.
     const LinTile c = lin_tile(p, tstart, unit);
     const bool f16 = p.q.f16 != 0;
-    const long long i = static_cast<long long>(c.ti) * p.feat + lane * 4;
+    const int f = threadIdx.x & 127;
+    const long long i = static_cast<long long>(c.ti) * p.feat + f;
     const int left = static_cast<int>(min(p.q.J - static_cast<long long>(c.tj) * p.bn, static_cast<long long>(p.bn)));
-    const int share = (left + p.split - 1) / p.split;
-    const int end = min(left, (static_cast<int>(rank) + 1) * share);
-    int col = static_cast<int>(rank) * share + warp;
+    const int share = split_share(left, p.split), first = static_cast<int>(rank) * share, end = min(left, first + share);
     const long long row0 = static_cast<long long>(c.tj) * p.bn;
-    float b0[4] = {}, b1[4] = {};
+    int col = first + 4 * (threadIdx.x >> 7);
+    float b0 = 0.0f, b1 = 0.0f;
     uint16_t res[4] = {};
-    if (col < end) {
+    const bool live = i < p.q.I;
+    auto residual = [&](int from) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (i + e < p.q.I) {
-          if (p.q.bias) {
-            b0[e] = from16(p.q.bias[i + e], f16);
-            if (FORM == FORM_GATED) b1[e] = from16(p.q.bias[p.q.I + i + e], f16);
-          }
-          if (p.q.residual) res[e] = p.q.residual[(row0 + col) * p.q.ldo + i + e];
-        }
-    }
-    cluster_sync_all();  // every CTA's partial sums are in its shared memory
-    for (; col < end; col += 8) {
-      float sum[2][4];
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[sub][e] = 0.0f;
-        if (sub >= SUBS) continue;
-        const uint32_t at = smem_base + ((sub * p.bn + col) * 128 + lane * 4) * 4;
-        float4 got[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r < p.split) got[r] = ld_cluster_f32x4(map_to_cta(at, r));
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r < p.split) {
-            sum[sub][0] += got[r].x;
-            sum[sub][1] += got[r].y;
-            sum[sub][2] += got[r].z;
-            sum[sub][3] += got[r].w;
-          }
+        if (from + e < end) res[e] = p.q.residual[(row0 + from + e) * p.q.ldo + i];
+    };
+    if (live && col < end) {
+      if (p.q.bias) {
+        b0 = from16(p.q.bias[i], f16);
+        if (FORM == FORM_GATED) b1 = from16(p.q.bias[p.q.I + i], f16);
       }
+      if (p.q.residual) residual(col);
+    }
+    cluster_wait();  // the partial sums of every CTA are here
+    const float4* inbox = reinterpret_cast<const float4*>(smem_raw + (smem_base - smem_u32(smem_raw)) + stages * stage_bytes);
+    for (; col < end; col += 8) {
+      float sum[2][4] = {};
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub)
+        for (int r = 0; r < p.split; ++r) {
+          const float4 got = inbox[((r * SUBS + sub) * (share >> 2) + ((col - first) >> 2)) * 128 + f];
+          sum[sub][0] += got.x;
+          sum[sub][1] += got.y;
+          sum[sub][2] += got.z;
+          sum[sub][3] += got.w;
+        }
+      if (!live) continue;
       uint16_t now[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        now[e] = res[e];
-        if (p.q.residual && col + 8 < end && i + e < p.q.I) res[e] = p.q.residual[(row0 + col + 8) * p.q.ldo + i + e];
-      }
-      lin_finish4<FORM == FORM_GATED>(p.q, sum[0], sum[1], b0, b1, now, i, row0 + col);
+      for (int e = 0; e < 4; ++e) now[e] = res[e];
+      if (p.q.residual && col + 8 < end) residual(col + 8);
+      lin_finish4<FORM == FORM_GATED>(p.q, sum[0], sum[1], b0, b1, now, i, row0 + col, end - col);
     }
   }
 
@@ -704,10 +753,11 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
+  if constexpr (SPLIT) return;  // nothing reads or writes this CTA's shared memory any more
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR || SPLIT) cluster_sync_all();  // shared memory and TMEM stay until every CTA is done
-  if (!SPLIT && warp == 1) {
+  if constexpr (PAIR) cluster_sync_all();  // shared memory and TMEM stay until both CTAs are done
+  if (warp == 1) {
     tc_fence_after();
     if constexpr (PAIR) tmem_dealloc_pair(tmem_base, p.tmem_cols);
     else tmem_dealloc(tmem_base, p.tmem_cols);
@@ -721,30 +771,57 @@ constexpr size_t kTwoCtas = 113 * 1024 - kStaticSmem;
 
 struct LinPick {
   bool pair;
-  int form, bn, split, stages;
+  int form, bn, split;
+  bool deep;  // single CTAs with an SM's shared memory each: no more of them than SMs, and clusters of at most four
+              // (eight such CTAs find room in a GPC twice at best: 22 us against 16 with four, 8 x 2048 x 8192)
 };
 
 static size_t stage_size(const LinPick& c) {
   return (c.form == FORM_PLAIN ? 1 : 2) * static_cast<size_t>(kSubBytes) + static_cast<size_t>(c.bn / (c.pair ? 2 : 1)) * 128;
 }
 
+// Shared memory behind the stages: the epilogue's staging, or the inbox of a split reduction.
+static size_t turn_bytes(const LinPick& c) {
+  if (c.split > 1) return static_cast<size_t>(c.split) * split_share(c.bn, c.split) * (c.form == FORM_PLAIN ? 1 : 2) * 128 * sizeof(float);
+  return static_cast<size_t>(c.pair ? 8 : 4) * kTurnFloats * sizeof(float);
+}
+
+static int max_stages(const LinPick& c) {
+  size_t n = 0;
+  if (!c.pair && !c.deep && kTwoCtas > 1024 + turn_bytes(c)) n = (kTwoCtas - 1024 - turn_bytes(c)) / stage_size(c);
+  if (n < 2) n = (kOneCta - 1024 - turn_bytes(c)) / stage_size(c);  // (also where two stages and a wide inbox need it)
+  return static_cast<int>(n < kLinStages ? n : kLinStages);
+}
+
+// Tiles of a product, at most: a group ends in at most one partial tile.
+static int64_t most_tiles(const LinArgs& q, const LinPick& c) {
+  const int64_t ti = ceil_div64(q.I, 128 * (c.pair ? 2 : 1) * (c.form == FORM_WIDE ? 2 : 1));
+  if (q.mode == LIN_ROWS) return (q.rows / c.bn + (q.groups < q.rows ? q.groups : q.rows)) * ti;
+  return ceil_div64(q.J, c.bn) * ti * (q.mode == LIN_REDUCE ? q.groups : 1);
+}
+
 // Time of a product under one variant, in SM cycles.  What the terms stand for, with what was measured:
-//   a stage costs its rows (128 bytes each) through the SM's port, 3.6 cycles a row, or its MMAs, the larger: bn / 2
-//   cycles of arithmetic per step of 16 and A sub-tile, but at least 137 per instruction of one issuing thread;
-//   rows fetched by number cost 45 cycles per four of them and loader warp;
-//   the epilogue issues about 12 instructions per result and warp, 16 more for an activation, 6 for a residual and for
-//   preact, half as many again in 2-byte accesses; it runs under the next tile's main loop where a second accumulator
-//   exists;
+//   a stage costs its rows (128 bytes each) through the SM's port, 2.65 cycles a row, its MMAs, bn / 2 cycles of
+//   arithmetic per step of 16 and A sub-tile (1.3 times that with two sub-tiles, which run into the power cap), its share
+//   of a copy's latency (2400 cycles over the stages in flight, half a stage less), or the hand-offs of one stage (500
+//   cycles in a pair, 420 alone), whichever is most; rows fetched by number cost 12 cycles each;
+//   no product is faster than its operands and results at the 3450 bytes a cycle of the memory;
+//   the epilogue costs a scheduler's warps in turn about 22 cycles per column, 16 more for an activation, 6 for a residual
+//   and for preact, half as many again in 2-byte accesses; it runs under the next tile's main loop where a second
+//   accumulator exists;
 //   a split reduction costs two cluster barriers and the exchange of its columns.
-static double variant_cycles(const LinArgs& q, const LinPick& c, int sms) {
+// Estimates against measurements: 1 x 4096 x 4096 split 8 / 4 / 2: 9.0 / 9.4 / 13.5 us measured; 256 x 4096 x 4096 pairs of
+// 64 / 256 tokens 20.8 / 25.5; 1237 x 2048 x 1000 pairs of 160 / 256 tokens 15.7 / 20.1, single CTAs of 96 tokens 21.4.
+static double variant_cycles(const LinArgs& q, LinPick c, int sms) {
+  c.deep = !c.pair && c.split <= 4 && most_tiles(q, c) * c.split <= sms;
   const double blocks = q.mode == LIN_REDUCE ? static_cast<double>(q.rows) / q.groups / kKBlock + 0.5
                                              : static_cast<double>(ceil_div64(q.K, kKBlock));
   const int subs = c.form == FORM_PLAIN ? 1 : 2, mult = (c.pair ? 2 : 1) * (c.form == FORM_WIDE ? 2 : 1);
   const double tiles_i = static_cast<double>(ceil_div64(q.I, 128 * mult));
+  const double busy = static_cast<double>(q.groups < q.rows ? q.groups : q.rows);
   double tiles;
   if (q.mode == LIN_ROWS) {
     // the rows of a group fill its tiles but for half of the last one
-    const double busy = static_cast<double>(q.groups < q.rows ? q.groups : q.rows);
     tiles = static_cast<double>(q.rows) / c.bn + 0.5 * busy;
     if (tiles < busy) tiles = busy;
   } else {
@@ -757,20 +834,26 @@ static double variant_cycles(const LinArgs& q, const LinPick& c, int sms) {
   if (q.mode != LIN_ROWS || waves < 1) waves = static_cast<double>(static_cast<int64_t>(waves + 0.999999));
   else waves += 0.5;
   const int bj = c.pair ? c.bn / 2 : c.bn;
-  double load = 3.6 * (128 * subs + bj) * per_sm;
-  if (q.mode == LIN_ROWS && q.gather_div && bj / 8 * 45.0 * 2 > load) load = bj / 8 * 45.0 * 2;
-  if (q.mode == LIN_REDUCE && q.gather_div) load += 8 * 2 * subs * 45.0;
-  const double math = 4.0 * subs * c.bn / 2 * per_sm;
-  const double stage = load > math ? (load > 548 ? load : 548) : (math > 548 ? math : 548);
+  double load = 2.65 * (128 * subs + bj);
+  if (q.mode == LIN_ROWS && q.gather_div) load += (12 - 2.65) * bj;
+  const double latency = 2400.0 / (max_stages(c) - 0.5), handoff = c.pair ? 500 : 420;
+  const double math = (subs == 2 ? 1.3 : 1.0) * 4.0 * subs * (c.bn / 2 > 64 ? c.bn / 2 : 64);
+  double stage = (load > math ? load : math) * per_sm;
+  if (stage < latency) stage = latency;
+  if (stage < handoff) stage = handoff;
   const double main_loop = static_cast<double>(static_cast<int64_t>(blocks / c.split + 0.999999)) * stage;
-  double per_col = 12 + (q.act ? 16 : 0) + (q.residual ? 6 : 0) + (q.preact ? 6 * subs : 0) + (q.gated ? 4 : 0);
+  double per_col = 22 + (q.act ? 16 : 0) + (q.residual ? 6 : 0) + (q.preact ? 6 * subs : 0) + (q.gated ? 8 : 0);
   if (q.I % 8) per_col *= 1.5;
-  // warps of a scheduler take turns; a pair's eight warps share the columns, or each sub-tile's four take all of them
+  // a pair's eight warps share the columns, or each sub-tile's four take all of them
   const double epi = c.pair ? per_col * (c.form == FORM_WIDE ? 2 * c.bn : c.bn) : per_col * c.bn * per_sm;
-  const bool covered = c.form == FORM_WIDE || c.form == FORM_PLAIN || (c.pair ? c.bn <= 128 : c.bn <= 64);
+  const bool covered = c.form == FORM_PLAIN || (c.form == FORM_GATED && (c.pair ? c.bn <= 128 : c.bn <= 64));
   const double tile = covered ? (main_loop > epi ? main_loop : epi) : main_loop + epi;
-  double total = 3000 + (waves - 1) * tile + main_loop + epi;
-  if (c.split > 1) total += 3000 + 60.0 * c.bn / c.split;
+  double body = (waves - 1) * tile + main_loop;
+  const double a_bytes = 2.0 * q.I * (q.gated ? 2 : 1) * (q.mode == LIN_REDUCE ? q.rows : q.K) * (q.mode == LIN_ROWS ? busy : 1);
+  const double memory = (a_bytes + 2.0 * q.J * q.I) / 3450;
+  if (body < memory) body = memory;
+  double total = 3000 + body + epi;
+  if (c.split > 1) total += 5000 + 220.0 * subs * (q.J < c.bn ? q.J : c.bn) / c.split;
   return total;
 }
 
@@ -817,9 +900,9 @@ static LinPick pick_variant(const LinArgs& q, int sms) {
   return best;
 }
 
-template <bool PAIR, int FORM, int EPI, bool SPLIT>
+template <bool PAIR, int FORM, int EPI, bool SPLIT, bool RICH>
 static int launch_variant(const LinMaps& maps, const LinUmma& p, int ctas, size_t smem, cudaStream_t stream) {
-  auto kern = linear_umma_kernel<PAIR, FORM, EPI, SPLIT>;
+  auto kern = linear_umma_kernel<PAIR, FORM, EPI, SPLIT, RICH>;
   static std::mutex mu;
   static bool done[64] = {false};
   int dev = 0;
@@ -858,11 +941,11 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
       }
     }
   }
-  const bool two = !c.pair;
-  const size_t turn = static_cast<size_t>(two ? 4 : 8) * kTurnFloats * sizeof(float);
-  const size_t limit = (two ? kTwoCtas : kOneCta) - 1024 - turn;
-  int stages = static_cast<int>(limit / stage_size(c));
-  if (stages > kLinStages) stages = kLinStages;
+  const int64_t most = most_tiles(q, c);
+  if (most > 0x7fffffffll / 8) return FTB_E_TOO_LARGE;
+  c.deep = !c.pair && c.split <= 4 && most * c.split <= sms;
+  const bool two = !c.pair && !c.deep;
+  int stages = max_stages(c);
   if (cfg && cfg->stages) {
     if (cfg->stages > stages) return FTB_E_BAD_CONFIG;
     stages = cfg->stages;
@@ -879,16 +962,16 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
   p.split = c.split;
   p.feat = c.form == FORM_WIDE ? 2 * m : m;
   p.sub_off = c.form == FORM_WIDE ? m : static_cast<int>(q.I);
-  const int64_t ti = ceil_div64(q.I, p.feat), tj = q.mode == LIN_ROWS ? 1 : ceil_div64(q.J, c.bn);
-  p.tiles_i = static_cast<int>(ti);
-  p.tiles_j = static_cast<int>(tj);
-  // the most tiles there can be: a group ends in at most one partial tile
-  const int64_t busy = q.mode == LIN_ROWS ? (q.groups < q.rows ? q.groups : q.rows) : 0;
-  const int64_t most = q.mode == LIN_ROWS ? (q.rows / c.bn + busy) * ti : ti * tj * (q.mode == LIN_REDUCE ? q.groups : 1);
-  if (most > 0x7fffffffll / 8) return FTB_E_TOO_LARGE;
+  p.tiles_i = static_cast<int>(ceil_div64(q.I, p.feat));
+  p.tiles_j = static_cast<int>(q.mode == LIN_ROWS ? 1 : ceil_div64(q.J, c.bn));
   p.band = 8;
+  p.by_i = fast_div(p.tiles_i);
+  p.by_group = fast_div(static_cast<int64_t>(p.tiles_i) * p.tiles_j);
+  p.by_span = fast_div(static_cast<int64_t>(p.tiles_i) * p.band);
+  p.by_band = fast_div(p.band);
+  p.by_last = fast_div(p.tiles_j % p.band ? p.tiles_j % p.band : p.band);
   const int acc_cols = subs * c.bn;
-  p.acc_slots = c.form == FORM_WIDE ? 2 : c.split > 1 || 2 * acc_cols > (two ? 256 : 512) ? 1 : 2;
+  p.acc_slots = c.form == FORM_WIDE ? 2 : c.split > 1 || 2 * acc_cols > (c.pair ? 512 : 256) ? 1 : 2;
   uint32_t cols = 32;
   while (cols < static_cast<uint32_t>(c.form == FORM_WIDE ? acc_cols : p.acc_slots * acc_cols)) cols *= 2;
   p.tmem_cols = cols;
@@ -919,12 +1002,11 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
     const uint64_t d[3] = {q.a_mn ? a_rows : kk, q.a_mn ? kk : a_rows, static_cast<uint64_t>(q.mode == LIN_ROWS ? q.groups : 1)};
     const uint32_t box[3] = {64, q.a_mn ? 64u : 128u, 1};
     const uint64_t st[2] = {static_cast<uint64_t>(q.lda) * 2, d[1] * static_cast<uint64_t>(q.lda) * 2};
-    if (!(reduce && gathers)) rc = make_tmap(&maps.a, dt, 3, q.a, d, st, box, ones);
+    rc = make_tmap(&maps.a, dt, 3, q.a, d, st, box, ones);
     if (!rc && reduce) {
-      const uint64_t src = static_cast<uint64_t>(gathers ? q.src_rows : q.rows), dr[2] = {a_rows, src};
-      const uint32_t row_box[2] = {64, 1};
-      rc = make_tmap(&maps.a_rows, dt, 2, q.a, dr, st, row_box, ones);
-      p.oob_a = static_cast<int>(src);
+      const uint32_t row_box[2] = {64, 1}, run_box[3] = {64, 16, 1};
+      rc = make_tmap(&maps.a_rows, dt, 2, q.a, d, st, row_box, ones);
+      if (!rc) rc = make_tmap(&maps.a16, dt, 3, q.a, d, st, run_box, ones);
     }
     if (rc) return rc;
   }
@@ -936,32 +1018,39 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
     const uint64_t st[2] = {static_cast<uint64_t>(q.ldb) * 2, d[1] * static_cast<uint64_t>(q.ldb) * 2};
     if (!(q.mode == LIN_ROWS && gathers)) rc = make_tmap(&maps.b, dt, 3, q.b, d, st, box, ones);
     if (!rc && (reduce || (q.mode == LIN_ROWS && gathers))) {
-      const uint32_t row_box[2] = {64, 1};
+      const uint32_t row_box[2] = {64, 1}, run_box[3] = {64, 16, 1};
       rc = make_tmap(&maps.b_rows, dt, 2, q.b, d, st, row_box, ones);
+      if (!rc && reduce) rc = make_tmap(&maps.b16, dt, 3, q.b, d, st, run_box, ones);
       p.oob_b = static_cast<int>(d[1]);
     }
     if (rc) return rc;
   }
 
-  size_t smem = static_cast<size_t>(stages) * stage_size(c) + 1024 + turn;
+  size_t smem = static_cast<size_t>(stages) * stage_size(c) + 1024 + turn_bytes(c);
   // A pair holds tensor memory while its CTAs wait for each other.  No other kernel with tensor memory may share the SM
   // with it (each could wait for columns that the other holds), so it always asks for most of the shared memory.
   if (c.pair && smem < 176 * 1024) smem = 176 * 1024;
+  const bool rich = q.gated || q.act || q.bias || q.residual || q.preact;
   if (c.split > 1) {
     const int ctas = static_cast<int>(most) * c.split;
-    return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, true>(maps, p, ctas, smem, stream)
-                                : launch_variant<false, FORM_PLAIN, 4, true>(maps, p, ctas, smem, stream);
+    return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, true, true>(maps, p, ctas, smem, stream)
+                                : launch_variant<false, FORM_PLAIN, 4, true, true>(maps, p, ctas, smem, stream);
   }
   if (c.pair) {
     const int64_t units = sms / 2 < most ? sms / 2 : most;
     const int ctas = static_cast<int>(units) * 2;
-    if (c.form == FORM_GATED) return launch_variant<true, FORM_GATED, 8, false>(maps, p, ctas, smem, stream);
-    if (c.form == FORM_WIDE) return launch_variant<true, FORM_WIDE, 8, false>(maps, p, ctas, smem, stream);
-    return launch_variant<true, FORM_PLAIN, 8, false>(maps, p, ctas, smem, stream);
+    if (c.form == FORM_GATED) return launch_variant<true, FORM_GATED, 8, false, true>(maps, p, ctas, smem, stream);
+    if (c.form == FORM_WIDE)
+      return rich ? launch_variant<true, FORM_WIDE, 8, false, true>(maps, p, ctas, smem, stream)
+                  : launch_variant<true, FORM_WIDE, 8, false, false>(maps, p, ctas, smem, stream);
+    return rich ? launch_variant<true, FORM_PLAIN, 8, false, true>(maps, p, ctas, smem, stream)
+                : launch_variant<true, FORM_PLAIN, 8, false, false>(maps, p, ctas, smem, stream);
   }
-  const int ctas = static_cast<int>(2 * sms < most ? 2 * sms : most);
-  return c.form == FORM_GATED ? launch_variant<false, FORM_GATED, 4, false>(maps, p, ctas, smem, stream)
-                              : launch_variant<false, FORM_PLAIN, 4, false>(maps, p, ctas, smem, stream);
+  const int64_t slots = two ? 2 * sms : sms;
+  const int ctas = static_cast<int>(slots < most ? slots : most);
+  if (c.form == FORM_GATED) return launch_variant<false, FORM_GATED, 4, false, true>(maps, p, ctas, smem, stream);
+  return rich ? launch_variant<false, FORM_PLAIN, 4, false, true>(maps, p, ctas, smem, stream)
+              : launch_variant<false, FORM_PLAIN, 4, false, false>(maps, p, ctas, smem, stream);
 }
 
 }  // namespace ftb

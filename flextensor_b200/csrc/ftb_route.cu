@@ -26,6 +26,7 @@ struct RouteArgs {
   void* dlogits;
   long long tokens;
   int experts, top_k, scoring, groups, top_groups, renorm, vec;
+  int group_lanes;  // lanes of a group where every lane's experts share one and the lanes are a power of two, else 0
   float scale;
 };
 
@@ -100,34 +101,27 @@ __device__ __forceinline__ uint64_t key_max(uint64_t k) {
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-// The `count` largest of the available values c, best first, ties to the lowest index: lane j gets the index of the
-// j-th.  `near` is set when two neighbours in that order, the last chosen and the first left out among them, are at
-// most `tol` apart.
-template <typename S, int VPL>
-__device__ __forceinline__ int pick(const S (&c)[VPL], uint32_t avail, int count, S tol, int lane, bool* near) {
+// The `count` largest of a lane's keys (0: not there), best first, ties to the lowest index: lane j gets the index of
+// the j-th.
+template <typename K, int VPL>
+__device__ __forceinline__ int pick(K (&k)[VPL], int count, int lane) {
   int mine = 0;
-  S prev = S(0);
-  for (int j = 0; j <= count; ++j) {
-    S best = S(0);
-    int at = -1;
+  for (int j = 0; j < count; ++j) {
+    K best = k[0];
+    int at = 0;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v)
-      if (((avail >> v) & 1u) && (at < 0 || c[v] > best)) {
-        best = c[v];
+    for (int v = 1; v < VPL; ++v)
+      if (k[v] > best) {
+        best = k[v];
         at = v;
       }
-    decltype(order_key(best)) key = 0;
-    if (at >= 0) key = order_key(best);
-    const auto top = key_max(key);
-    if (top == 0) break;  // none left
-    const S cur = key_value(top);
-    if (j > 0 && prev - cur <= tol) *near = true;
-    prev = cur;
-    if (j == count) break;
-    const int winner = __ffs(__ballot_sync(kAll, key == top)) - 1;
+    const K top = key_max(best);
+    const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
     const int id = __shfl_sync(kAll, lane * VPL + at, winner);
-    if (lane == winner) avail &= ~(1u << at);
     if (lane == j) mine = id;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (lane == winner && v == at) k[v] = 0;
   }
   return mine;
 }
@@ -141,42 +135,64 @@ __device__ __forceinline__ void merge_top2(S& a, S& b, S oa, S ob) {
   b = b > lo ? b : lo;
 }
 
+// The best top_groups of the values that the lanes hold (`there`: the lane holds one), as a mask of lanes; ties to the
+// lowest lane.  `near` is set where the last kept and the first left out are within `tol`.
+template <typename S>
+__device__ __forceinline__ uint32_t best_lanes(S value, bool there, int count, S tol, int lane, bool* near) {
+  if (value != value) value = static_cast<S>(-INFINITY);
+  auto key = order_key(value);
+  if (!there) key = 0;
+  auto last = key;
+  uint32_t kept = 0;
+  for (int j = 0; j < count; ++j) {
+    last = key_max(key);
+    const uint32_t tied = __ballot_sync(kAll, key == last), lowest = tied & (0u - tied);
+    kept |= lowest;
+    if ((lowest >> lane) & 1u) key = 0;
+  }
+  const auto rest = key_max(key);
+  if (rest != 0) *near |= key_value(last) - key_value(rest) <= tol;
+  return kept;
+}
+
 // Bits of the lane's values that lie in the kept groups.
 template <typename S, int VPL>
 __device__ __forceinline__ uint32_t keep_groups(const RouteArgs& p, const S (&c)[VPL], uint32_t avail, S tol, int lane,
                                                 bool* near) {
-  const int size = p.experts / p.groups, e0 = lane * VPL;
   const S none = static_cast<S>(-INFINITY);
-  S value = none;  // of group `lane`
-  const int lanes = size / VPL;
-  if (size % VPL == 0 && (lanes & (lanes - 1)) == 0) {
-    // a lane's values share a group, a group is a run of 2^n lanes
+  if (p.group_lanes > 0) {
+    // a group is a run of lanes
     S a = none, b = none;
 #pragma unroll
     for (int v = 0; v < VPL; ++v)
       if ((avail >> v) & 1u) merge_top2(a, b, c[v], none);
-    for (int d = 1; d < lanes; d <<= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
-    const S sum = size > 1 ? a + b : a;
-    value = __shfl_sync(kAll, sum, lane < p.groups ? lane * lanes : 0);
-  } else {
-    for (int g = 0; g < p.groups; ++g) {
-      S a = none, b = none;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v)
-        if (((avail >> v) & 1u) && (e0 + v) / size == g) merge_top2(a, b, c[v], none);
-#pragma unroll
-      for (int d = 16; d; d >>= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
-      if (lane == g) value = size > 1 ? a + b : a;
-    }
+    for (int d = 1; d < p.group_lanes; d <<= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
+    const int first = lane & ~(p.group_lanes - 1);
+    const uint32_t kept = best_lanes<S>(p.group_lanes * VPL > 1 ? a + b : a, lane == first && lane * VPL < p.experts, p.top_groups, tol, lane, near);
+    return (kept >> first) & 1u ? avail : 0u;
   }
-  if (value != value) value = none;
-  const S one[1] = {value};
-  const int mine = pick<S, 1>(one, lane < p.groups ? 1u : 0u, p.top_groups, 2 * tol, lane, near);
-  uint32_t kept = __reduce_or_sync(kAll, lane < p.top_groups ? 1u << mine : 0u);
-  uint32_t left = 0;
+  const int size = p.experts / p.groups, e0 = lane * VPL;
+  S value = none;  // of group `lane`
+  for (int g = 0; g < p.groups; ++g) {
+    S a = none, b = none;
 #pragma unroll
-  for (int v = 0; v < VPL; ++v)
-    if (((avail >> v) & 1u) && ((kept >> ((e0 + v) / size)) & 1u)) left |= 1u << v;
+    for (int v = 0; v < VPL; ++v)
+      if (((avail >> v) & 1u) && e0 + v >= g * size && e0 + v < (g + 1) * size) merge_top2(a, b, c[v], none);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
+    if (lane == g) value = size > 1 ? a + b : a;
+  }
+  const uint32_t kept = best_lanes<S>(value, lane < p.groups, p.top_groups, tol, lane, near);
+  uint32_t left = 0;
+  int g = e0 / size, end = (g + 1) * size;
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) {
+    if (e0 + v >= end) {
+      ++g;
+      end += size;
+    }
+    if (((avail >> v) & 1u) && ((kept >> g) & 1u)) left |= 1u << v;
+  }
   return left;
 }
 
@@ -185,8 +201,12 @@ __device__ __forceinline__ float exp_below(float x, float m) { return m == -INFI
 
 template <int VPL>
 __device__ __noinline__ int choose_exactly(const RouteArgs& p, const float (&x)[VPL], uint32_t avail, float m, int lane) {
-  bool near = false;
-  if (!p.bias && p.groups == 1) return pick<float, VPL>(x, avail, p.top_k, -1.0f, lane, &near);
+  if (!p.bias && p.groups == 1) {
+    uint32_t k[VPL];
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) k[v] = (avail >> v) & 1u ? order_key(x[v]) : 0u;
+    return pick<uint32_t, VPL>(k, p.top_k, lane);
+  }
   double c[VPL];
   double sum = 0.0;
   const int e0 = lane * VPL;
@@ -204,8 +224,12 @@ __device__ __noinline__ int choose_exactly(const RouteArgs& p, const float (&x)[
     if (p.bias && ((avail >> v) & 1u)) c[v] += static_cast<double>(p.bias[e0 + v]);
     c[v] = c[v] != c[v] ? -INFINITY : c[v] + 0.0;
   }
+  bool near = false;
   if (p.groups > 1) avail = keep_groups<double, VPL>(p, c, avail, -1.0, lane, &near);
-  return pick<double, VPL>(c, avail, p.top_k, -1.0, lane, &near);
+  uint64_t k[VPL];
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) k[v] = (avail >> v) & 1u ? order_key(c[v]) : 0ull;
+  return pick<uint64_t, VPL>(k, p.top_k, lane);
 }
 
 // Batcher's odd-even merge sort of N keys in registers, largest first.
@@ -226,21 +250,18 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
           }
 }
 
-// pick() on sorted keys.  `tol` < 0: values that agree in every bit but the place's are near where `exact` is false.
+// pick() on sorted keys; `gap` becomes the least distance between neighbours in the order of choice, the last chosen and
+// the first left out among them (0 for values that differ in the place's bits only).
 template <int VPL>
-__device__ __forceinline__ int pick_sorted(uint32_t (&k)[VPL], int count, float tol, bool exact, int lane, bool* near) {
+__device__ __forceinline__ int pick_sorted(uint32_t (&k)[VPL], int count, int lane, float* gap) {
   constexpr uint32_t PLACE = VPL - 1;
   int mine = 0;
-  uint32_t prev = 0;
-  for (int j = 0; j <= count; ++j) {
+  float prev = INFINITY, least = INFINITY;
+  for (int j = 0; j < count; ++j) {
     const uint32_t head = k[0] & ~PLACE, top = __reduce_max_sync(kAll, head);
-    if (top == 0) break;  // none left
-    if (j > 0) {
-      if (tol < 0.0f) *near |= !exact && prev == top;
-      else *near |= key_value(prev) - key_value(top) <= tol;
-    }
-    prev = top;
-    if (j == count) break;
+    const float cur = key_value(top);
+    least = fminf(least, prev - cur);
+    prev = cur;
     const int winner = __ffs(__ballot_sync(kAll, head == top)) - 1;
     const int id = __shfl_sync(kAll, lane * VPL + static_cast<int>(PLACE - (k[0] & PLACE)), winner);
     if (lane == j) mine = id;
@@ -250,10 +271,27 @@ __device__ __forceinline__ int pick_sorted(uint32_t (&k)[VPL], int count, float 
       k[VPL - 1] = 0;
     }
   }
+  const uint32_t rest = __reduce_max_sync(kAll, k[0] & ~PLACE);
+  if (rest != 0) least = fminf(least, prev - key_value(rest));
+  *gap = least;
   return mine;
 }
 
-template <typename T, int VPL>
+// The groups kept, where a group is a run of p.group_lanes lanes: from the two largest keys of every lane.  Returns
+// whether the lane's group stays; `near` where the last group kept and the first left out are within `tol`.
+template <int VPL>
+__device__ __forceinline__ bool keep_lane_groups(const RouteArgs& p, const uint32_t (&k)[VPL], float tol, int lane, bool* near) {
+  constexpr uint32_t PLACE = VPL - 1;
+  // (the key of -inf without its place's bits is none: clean)
+  float a = clean(key_value(k[0] & ~PLACE)), b = VPL > 1 ? clean(key_value(k[VPL > 1 ? 1 : 0] & ~PLACE)) : -INFINITY;
+  for (int d = 1; d < p.group_lanes; d <<= 1) merge_top2(a, b, __shfl_xor_sync(kAll, a, d), __shfl_xor_sync(kAll, b, d));
+  const int first = lane & ~(p.group_lanes - 1);
+  const uint32_t kept = best_lanes<float>(p.group_lanes * VPL > 1 ? a + b : a, lane == first && lane * VPL < p.experts, p.top_groups, tol, lane, near);
+  return (kept >> first) & 1u;
+}
+
+// FULL: every lane has VPL experts, and the rows and the bias can be read in 16-byte words.
+template <typename T, int VPL, bool FULL>
 __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
@@ -263,14 +301,13 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
   const T* row = static_cast<const T*>(p.logits) + t * p.experts;
   const int e0 = lane * VPL;
   float x[VPL];
-  load_row<T, VPL>(row, p.experts, lane, p.vec != 0, x);
-  const int have = min(max(p.experts - e0, 0), VPL);
+  load_row<T, VPL>(row, p.experts, lane, FULL || p.vec != 0, x);
+  const int have = FULL ? VPL : min(max(p.experts - e0, 0), VPL);
   const uint32_t avail = have >= 32 ? kAll : (1u << have) - 1u;
 
   const bool sigmoid = p.scoring == FTB_SCORE_SIGMOID;
   const bool by_logit = !p.bias && p.groups == 1;
   float m = -INFINITY, total = 0.0f;
-  const bool need_sum = !sigmoid && (!by_logit || !p.renorm);
   if (!sigmoid) {
 #pragma unroll
     for (int v = 0; v < VPL; ++v) m = fmaxf(m, x[v]);
@@ -278,54 +315,66 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
   }
   constexpr uint32_t PLACE = VPL - 1;
   uint32_t k[VPL];
-  bool near = false;
   int mine;
+  bool near = false;
   if (by_logit) {
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) k[v] = ((avail >> v) & 1u) ? (order_key(x[v]) & ~PLACE) | (PLACE - v) : 0u;
+    for (int v = 0; v < VPL; ++v) k[v] = FULL || v < have ? (order_key(x[v]) & ~PLACE) | (PLACE - v) : 0u;
     sort_keys<VPL>(k);
-    // a 16-bit logit has no bits where the place goes
-    mine = pick_sorted<VPL>(k, p.top_k, -1.0f, sizeof(T) == 2 || VPL == 1, lane, &near);
-    if (need_sum) {
+    float gap;
+    mine = pick_sorted<VPL>(k, p.top_k, lane, &gap);
+    // A 16-bit logit has no bits where the place goes, so equal keys are equal logits.  An fp32 one may differ in the
+    // bits that the place took, and a difference with an infinity is not a number: look again.
+    if (sizeof(T) == 4 && VPL > 1) near = !(gap > 0.0f);
+    if (!sigmoid && !p.renorm) {
 #pragma unroll
       for (int v = 0; v < VPL; ++v) total += exp_below(x[v], m);
       total = warp_sum(total);
     }
   } else {
     float c[VPL];
-    float most = 0.0f;  // largest magnitude that enters a sum: what the error bound scales with
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
       c[v] = sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x[v])) : exp_below(x[v], m);
-      if (!sigmoid) total += ((avail >> v) & 1u) ? c[v] : 0.0f;
+      if (!FULL && v >= have) c[v] = 0.0f;
     }
-    float inv = 1.0f;
     if (!sigmoid) {
-      total = warp_sum(total);
-      inv = total > 0.0f ? 1.0f / total : 0.0f;
-    }
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      if (!sigmoid) c[v] *= inv;
-      const bool have_v = (avail >> v) & 1u;
-      if (have_v) most = fmaxf(most, c[v]);
-      if (p.bias && have_v) {
-        const float b = p.bias[e0 + v];
-        c[v] += b;
-        if (fabsf(b) < INFINITY) most = fmaxf(most, fabsf(b));
+      for (int v = 0; v < VPL; ++v) total += c[v];
+      total = warp_sum(total);
+      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) c[v] *= inv;
+    }
+    float most = 0.0f;  // largest magnitude that enters a sum: what the error bound scales with
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) most = fmaxf(most, c[v]);
+    if (p.bias) {
+      float b[VPL];
+      load_row<float, VPL>(p.bias, p.experts, lane, FULL, b);
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        const float size = fabsf(b[v]);
+        most = fmaxf(most, size < INFINITY ? size : 0.0f);
+        c[v] = clean(c[v] + b[v]);
       }
-      c[v] = clean(c[v]);
     }
     // The exponentials and reciprocals are good to a few units of 2^-24 of the largest score (their error grows with
     // |x|, where the score's slope has vanished faster), a sum over the row to about 8 more, and the place takes
     // VPL units of a value of up to twice that.
     const float tol = (3e-6f + VPL * 2.4e-7f) * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(most)));
     uint32_t left = avail;
-    if (p.groups > 1) left = keep_groups<float, VPL>(p, c, avail, tol, lane, &near);
+    if (p.groups > 1 && p.group_lanes == 0) left = keep_groups<float, VPL>(p, c, avail, 2.0f * tol, lane, &near);
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) k[v] = ((left >> v) & 1u) ? (order_key(c[v]) & ~PLACE) | (PLACE - v) : 0u;
+    for (int v = 0; v < VPL; ++v) k[v] = (left >> v) & 1u ? (order_key(c[v]) & ~PLACE) | (PLACE - v) : 0u;
     sort_keys<VPL>(k);
-    mine = pick_sorted<VPL>(k, p.top_k, tol, false, lane, &near);
+    if (p.groups > 1 && p.group_lanes > 0 && !keep_lane_groups<VPL>(p, k, 2.0f * tol, lane, &near)) {
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) k[v] = 0;
+    }
+    float gap;
+    mine = pick_sorted<VPL>(k, p.top_k, lane, &gap);
+    near |= !(gap > tol);
   }
   if (near) mine = choose_exactly<VPL>(p, x, avail, m, lane);
 
@@ -453,7 +502,9 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) 
 template <typename T, int VPL>
 static int launch_route(const RouteArgs& p, bool backward, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.tokens + 7) / 8));
-  return launch_overlapped(backward ? route_backward_kernel<T, VPL> : route_kernel<T, VPL>, grid, dim3(256), 0, 1, stream, p);
+  const bool full = p.experts == 32 * VPL && p.vec && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+  auto kern = backward ? route_backward_kernel<T, VPL> : full ? route_kernel<T, VPL, true> : route_kernel<T, VPL, false>;
+  return launch_overlapped(kern, grid, dim3(256), 0, 1, stream, p);
 }
 
 template <typename T>
@@ -515,6 +566,10 @@ int ftb_route_experts(int dtype, const void* logits, const float* bias, int32_t*
   p.top_groups = top_groups;
   p.renorm = renormalize != 0;
   p.scale = scale;
+  int vpl = 1;  // experts per lane, as run_route picks it
+  while (vpl * 32 < experts) vpl *= 2;
+  const int lanes = static_cast<int>(experts / groups) / vpl;
+  p.group_lanes = (experts / groups) % vpl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
   return run_route(dtype, p, false, static_cast<cudaStream_t>(stream));
 }
 

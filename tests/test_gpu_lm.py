@@ -304,7 +304,7 @@ def route64(logits, top_k, bias, scoring, groups, top_groups, renorm, scale):
         c = torch.where(logits.isnan(), -math.inf, logits.double())
     if groups > 1:
         part = c.view(t, groups, -1)
-        value = part.sort(dim=2, descending=True).values[:, :, :2].sum(2)
+        value = part.sort(dim=2, descending=True).values[:, :, :2].sum(2).clamp(min=-1e200)
         keep = value.sort(dim=1, descending=True, stable=True).indices[:, :top_groups]
         mask = torch.zeros(t, groups, dtype=torch.bool, device=c.device).scatter_(1, keep, True)
         c = torch.where(mask.repeat_interleave(e // groups, 1), c, torch.nan)
@@ -357,6 +357,21 @@ def test_route_near_ties(B, scoring, groups, top_groups):
         # equal logits give equal scores on both sides; unequal ones differ by 2^-24 of a score, far above 2^-53
         assert torch.equal(ids, want_ids)
         bounded(weights, want, 64 * E * want.abs(), "weights")
+
+
+@pytest.mark.parametrize("e,k,groups,top_groups", [(64, 6, 1, 1), (256, 8, 8, 4), (60, 5, 4, 2), (100, 9, 1, 1), (32, 4, 32, 6)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_bias_disables_experts(B, e, k, groups, top_groups, scoring):
+    """A bias of -inf: the expert is taken only when no other is left."""
+    t = 40
+    logits, bias = rand(e, t, e, dtype=torch.float32), rand(1, e, scale=0.1, dtype=torch.float32)
+    bias[::3] = -math.inf
+    bias[e // 2:e // 2 + 4] = -math.inf
+    ids, weights = torch.empty(t, k, device="cuda", dtype=torch.int32), torch.empty(t, k, device="cuda")
+    B.route_experts(logits, ids, weights, bias=bias, scoring=scoring, groups=groups, top_groups=top_groups, renormalize=False)
+    want_ids, want = route64(logits, k, bias, scoring, groups, top_groups, False, 1.0)
+    assert torch.equal(ids, want_ids)
+    bounded(weights, want, (32 + e / 8) * E * want.abs() + 1e-37, "weights")
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
