@@ -805,6 +805,17 @@ class ExpertPlan(object):
         self.slots = torch.full((self.rows,), -1, dtype=torch.int32, device=device)
         self.device = self.offsets.device
 
+    @classmethod
+    def over(cls, tokens, top_k, experts, offsets, order, slots):
+        """A plan whose buffers the caller owns."""
+        plan = cls.__new__(cls)
+        plan.tokens, plan.top_k, plan.experts, plan.rows = tokens, top_k, experts, tokens * top_k
+        for name, t, n in (("offsets", offsets, experts + 1), ("order", order, plan.rows), ("slots", slots, plan.rows)):
+            if _fits(t, name, (n,), torch.int32, offsets.device) is None:
+                raise TypeError("%s must be a CUDA tensor" % name)
+        plan.offsets, plan.order, plan.slots, plan.device = offsets, order, slots, offsets.device
+        return plan
+
 
 def _plan_of(plan):
     if not isinstance(plan, ExpertPlan):

@@ -105,12 +105,13 @@ class ComputeOp(Operation):
     """One stage of the graph.
 
     kind  : 'pad2d' | 'gemm' | 'batch_gemm' | 'gemm_int8' | 'conv2d' | 'depthwise_conv2d' |
-            'bias_add'
+            'bias_add' | 'linear' | 'route_experts' | 'expert_plan' | 'expert_linear' | 'expert_combine'
     attrs : kind-specific parameters (stride, padding, transposes, ...)
     axis / reduce_axis : loop axes with the names and extents the reference's lambdas have
+    more_outputs : (shape, dtype) of the outputs after the first
     """
 
-    def __init__(self, kind, name, out_shape, dtype, inputs, axis_names, reduce_axes=(), attrs=None):
+    def __init__(self, kind, name, out_shape, dtype, inputs, axis_names, reduce_axes=(), attrs=None, more_outputs=()):
         super().__init__(name)
         self.kind = kind
         self.attrs = dict(attrs or {})
@@ -119,6 +120,9 @@ class ComputeOp(Operation):
         self.axis = [IterVar(n, int(e)) for n, e in zip(axis_names, out_shape)]
         self.reduce_axis = list(reduce_axes)
         self._outputs = [Tensor(out_shape, dtype, self, 0, name)]
+        for i, (shape, kind_of) in enumerate(more_outputs):
+            self._outputs.append(Tensor(shape, kind_of, self, i + 1, "%s.%d" % (name, i + 1)))
+        self.num_outputs = len(self._outputs)
 
     @property
     def input_tensors(self):

@@ -1,4 +1,4 @@
-"""Compute definitions of the five hot-path operators, PyTorch conventions.
+"""Compute definitions of the hot-path operators, PyTorch conventions.
 
 Each function returns the output ``Tensor`` of a small op graph (see ``ir.py``), with the
 same argument meaning, shape checks, loop-axis names and output-size formulas as the
@@ -16,6 +16,9 @@ reference's ``flextensor/nn/ops.py``:
   gemm                   ops.py:1074-1108 (four transpose variants)
   batch_gemm             ops.py:1111-1158
   gemm_int8              no ops.py symbol; contract of test/test_tvm/legacy/gemm_int8.py:15-21
+  linear, route_experts, expert_plan, expert_linear, expert_combine
+                         no counterpart: the feed-forward operators of language models (matrix product
+                         with bias, activation, gate and residual; routing to experts and their products)
 
 The reference is fp32 only; ``dtype`` follows the input tensors here so that the same
 index expressions serve bf16 (fp32 accumulate) and int8 (int32 accumulate).
@@ -291,4 +294,98 @@ def gemm_int8(A, B, transposeA=False, transposeB=False):
     rk = reduce_axis((0, k), name="k")
     op = ComputeOp("gemm_int8", "compute", (m, n), "int32", [A, B], ("i", "j"), reduce_axes=[rk],
                    attrs={"transposeA": bool(transposeA), "transposeB": bool(transposeB)})
+    return op.output(0)
+
+
+# ---------------------------------------------------------------- feed-forward operators of language models
+_ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu")
+
+
+def _operands(**named):
+    """(names, tensors) of the operands that are given, in order."""
+    given = [(name, t) for name, t in named.items() if t is not None]
+    return tuple(name for name, _ in given), [t for _, t in given]
+
+
+def _product_dims(x, weight, bias, residual, activation, gated, lead):
+    """(rows, N, K) of a product with an epilogue; ``lead``: leading dimensions of weight and bias."""
+    rows, k = (int(s) for s in x.shape)
+    shape = [int(s) for s in weight.shape]
+    assert_print(len(shape) == len(lead) + 2 and shape[:-2] == lead and shape[-1] == k,
+                 "weight of shape %s for rows of %d" % (shape, k))
+    assert_print(activation in _ACTIVATIONS, "activation must be one of %s" % (_ACTIVATIONS,))
+    assert_print(x.dtype in ("bfloat16", "float16") and weight.dtype == x.dtype, "x and weight are bfloat16 or float16")
+    wide = shape[-2]
+    assert_print(not gated or wide % 2 == 0, "a gated weight has an even number of rows")
+    n = wide // 2 if gated else wide
+    if bias is not None:
+        assert_print([int(s) for s in bias.shape] == lead + [wide] and bias.dtype == x.dtype, "bias of shape %s" % (bias.shape,))
+    if residual is not None:
+        assert_print([int(s) for s in residual.shape] == [rows, n] and residual.dtype == x.dtype, "residual of shape %s" % (residual.shape,))
+    return rows, n, k
+
+
+def linear(x, weight, bias=None, residual=None, activation="none", gated=False):
+    """out[t,i] = act(sum_k x[t,k] * weight[i,k] + bias[i]) + residual[t,i]; ``gated``: weight [2N,K] holds the gate rows,
+    then the others, out = act(gate) * other + residual.  bfloat16 or float16, one kernel."""
+    t, n, k = _product_dims(x, weight, bias, residual, activation, gated, [])
+    names, tensors = _operands(x=x, weight=weight, bias=bias, residual=residual)
+    op = ComputeOp("linear", "linear", (t, n), x.dtype, tensors, ("t", "i"), reduce_axes=[reduce_axis((0, k), name="k")],
+                   attrs={"operands": names, "activation": activation, "gated": bool(gated)})
+    return op.output(0)
+
+
+def route_experts(logits, top_k, bias=None, scoring="softmax", groups=1, top_groups=1, renormalize=True, scale=1.0):
+    """(ids, weights), both [T, top_k]: the experts of every token and their weights (``backend.route_experts``)."""
+    t, e = (int(s) for s in logits.shape)
+    assert_print(1 <= top_groups <= groups and e % groups == 0 and 1 <= top_k <= e // groups * top_groups,
+                 "top_k %d of %d experts in %d groups, %d kept" % (top_k, e, groups, top_groups))
+    assert_print(scoring in ("softmax", "sigmoid"), "scoring must be softmax or sigmoid")
+    names, tensors = _operands(logits=logits, bias=bias)
+    op = ComputeOp("route_experts", "route_experts", (t, top_k), "int32", tensors, ("t", "j"),
+                   attrs={"operands": names, "scoring": scoring, "groups": int(groups), "top_groups": int(top_groups),
+                          "renormalize": bool(renormalize), "scale": float(scale)},
+                   more_outputs=[((t, top_k), "float32")])
+    return op.output(0), op.output(1)
+
+
+def expert_plan(ids, experts):
+    """(offsets [experts+1], order [T*top_k], slots [T*top_k]): rows of ids [T, top_k] sorted by expert."""
+    t, top_k = (int(s) for s in ids.shape)
+    assert_print(ids.dtype == "int32", "ids are int32")
+    op = ComputeOp("expert_plan", "expert_plan", (experts + 1,), "int32", [ids], ("e",),
+                   attrs={"tokens": t, "top_k": top_k, "experts": int(experts)},
+                   more_outputs=[((t * top_k,), "int32"), ((t * top_k,), "int32")])
+    return op.output(0), op.output(1), op.output(2)
+
+
+def _plan_attrs(plan):
+    assert_print(len(plan) == 3 and getattr(plan[0].op, "kind", None) == "expert_plan", "plan is what expert_plan returned")
+    return dict(plan[0].op.attrs)
+
+
+def expert_linear(x, weight, plan, bias=None, activation="none", gated=False, gather=False):
+    """out[p,i] for every sorted place p of expert e: the epilogue of ``linear`` over its row times weight[e] ([E,N,K], gated
+    [E,2N,K]) plus bias[e].  ``gather``: x is [T,K], read by token; else [T*top_k,K], sorted."""
+    sizes = _plan_attrs(plan)
+    rows, n, k = _product_dims(x, weight, bias, None, activation, gated, [sizes["experts"]])
+    assert_print(rows == (sizes["tokens"] if gather else sizes["tokens"] * sizes["top_k"]), "x has %d rows" % rows)
+    names, tensors = _operands(x=x, weight=weight, bias=bias)
+    op = ComputeOp("expert_linear", "expert_linear", (sizes["tokens"] * sizes["top_k"], n), x.dtype, tensors + list(plan),
+                   ("p", "i"), reduce_axes=[reduce_axis((0, k), name="k")],
+                   attrs={"operands": names + ("offsets", "order", "slots"), "activation": activation, "gated": bool(gated),
+                          "gather": bool(gather), **sizes})
+    return op.output(0)
+
+
+def expert_combine(y, plan, weights=None, residual=None):
+    """out[t,i] = residual[t,i] + sum_j weights[t,j] * y[place of (t, j), i]; dropped rows add nothing."""
+    sizes = _plan_attrs(plan)
+    rows, n = (int(s) for s in y.shape)
+    t, top_k = sizes["tokens"], sizes["top_k"]
+    assert_print(rows == t * top_k, "y has %d rows" % rows)
+    names, tensors = _operands(y=y, weights=weights, residual=residual)
+    op = ComputeOp("expert_combine", "expert_combine", (t, n), y.dtype, tensors + list(plan), ("t", "i"),
+                   reduce_axes=[reduce_axis((0, top_k), name="j")],
+                   attrs={"operands": names + ("offsets", "order", "slots"), **sizes})
     return op.output(0)

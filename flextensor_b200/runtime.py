@@ -31,7 +31,10 @@ from . import backend
 from .templates import config_to_knobs
 from .utils import Config, to_tuple
 
-_TORCH_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int8": torch.int8, "int32": torch.int32}
+_TORCH_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16, "int8": torch.int8,
+                 "int32": torch.int32}
+
+FEED_FORWARD = ("linear", "route_experts", "expert_plan", "expert_linear", "expert_combine")
 
 DEFAULT_PRECISION = {"gemm": "3xtf32", "batch_gemm": "3xtf32", "conv2d": "tf32"}
 
@@ -189,6 +192,30 @@ class Module(object):
             self._packed[idx] = (weight, weight._version, ws)
         return packed
 
+    def _run_feed_forward(self, op, ins, outs, cfg, status):
+        """One of the feed-forward operators: operands by name, every output an array of ``bufs``."""
+        attrs = op.attrs
+        named = dict(zip(attrs.get("operands", ()), ins))
+        plan = None
+        if op.kind in ("expert_linear", "expert_combine"):
+            plan = backend.ExpertPlan.over(attrs["tokens"], attrs["top_k"], attrs["experts"], named["offsets"], named["order"],
+                                           named["slots"])
+        if op.kind == "linear":
+            backend.linear(named["x"], named["weight"], outs[0], bias=named.get("bias"), residual=named.get("residual"),
+                           activation=attrs["activation"], gated=attrs["gated"], cfg=cfg, status=status)
+        elif op.kind == "route_experts":
+            backend.route_experts(named["logits"], outs[0], outs[1], bias=named.get("bias"), scoring=attrs["scoring"],
+                                  groups=attrs["groups"], top_groups=attrs["top_groups"], renormalize=attrs["renormalize"],
+                                  scale=attrs["scale"])
+        elif op.kind == "expert_plan":
+            backend.expert_plan(ins[0], backend.ExpertPlan.over(attrs["tokens"], attrs["top_k"], attrs["experts"], *outs))
+        elif op.kind == "expert_linear":
+            backend.expert_linear(named["x"], named["weight"], plan, outs[0], bias=named.get("bias"),
+                                  activation=attrs["activation"], gated=attrs["gated"], gather=attrs["gather"], cfg=cfg,
+                                  status=status)
+        else:
+            backend.expert_combine(named["y"], plan, outs[0], weights=named.get("weights"), residual=named.get("residual"))
+
     def __call__(self, *arrays):
         table = self._bind(arrays)
         device = arrays[-1].device
@@ -276,6 +303,12 @@ class Module(object):
                 else:
                     backend.dwconv2d_nchw_f32(ins[0], ins[1], out, bias, op.attrs["stride"], op.attrs["padding"],
                                               op.attrs["dilation"], cfg=cfg, status=status)
+            elif op.kind in FEED_FORWARD:
+                try:
+                    outs = [table[id(op.output(i))] for i in range(op.num_outputs)]
+                except KeyError:
+                    raise RuntimeError("every output of %s must be one of bufs" % op.kind)
+                self._run_feed_forward(op, ins, outs, cfg, status)
             else:
                 raise RuntimeError("no kernel for op kind %r" % (op.kind,))
             if peers and len(peers) > 1:

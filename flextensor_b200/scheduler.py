@@ -52,7 +52,21 @@ def flatten_graph(ops):
                 queue.append(t.op)
             down_graph.setdefault(t, []).append(cur)
     order.reverse()
-    return order, down_graph
+    # Breadth first from the outputs puts producers first in a chain; where an op is reached over paths of different
+    # lengths, the ops that are not ready yet wait for their producers.
+    ready, sorted_order = set(), []
+    known = {id(op) for op in order}
+    while order:
+        waiting = []
+        for op in order:
+            if all(id(t.op) in ready or id(t.op) not in known for t in op.input_tensors):
+                ready.add(id(op))
+                sorted_order.append(op)
+            else:
+                waiting.append(op)
+        assert_print(len(waiting) < len(order), "the graph has a cycle")
+        order = waiting
+    return sorted_order, down_graph
 
 
 class OpState(object):

@@ -295,6 +295,8 @@ B200_LAYOUT = {
     "conv2d": {"spatial": ["tile_n", "tile_h", "cluster"], "reduce": ["stages", "split_k"], "reorder": ["raster"],
                "unroll": ["ctas"], "inline": ["algo"]},
     "depthwise_conv2d": {"spatial": ["tile_h", "threads"], "reduce": [], "reorder": [], "unroll": []},
+    # products with an epilogue; 0 leaves a knob to the library's choice
+    "linear": {"spatial": ["tile_n", "cluster"], "reduce": ["stages", "split_k"], "reorder": [], "unroll": []},
 }
 
 _ELEM_BYTES = {"float32": 4, "bfloat16": 2, "int8": 1}
@@ -306,6 +308,8 @@ def op_family(op):
         return "contraction"
     if kind in ("conv2d", "depthwise_conv2d"):
         return kind
+    if kind in ("linear", "expert_linear"):
+        return "linear"
     return None
 
 
@@ -395,6 +399,13 @@ def generate_space_intra_op_b200(op, down_graph=None):
         elif form == "nhwc":
             algos = [1] + ([2, 5] if slab_ok else [])  # read in place: no NCHW batched GEMM, no im2col form
         space.add_subspace("algo", KnobSpace("algo", algos), "inline")
+    elif family == "linear":
+        # tokens per tile; a pair tile has 128 or 256 of them, a split reduction at most 64
+        space.add_subspace("tile_n", KnobSpace("tile_n", [0, 16, 32, 64, 128, 256]), "spatial")
+        space.add_subspace("cluster", KnobSpace("cluster", [0, 1, 2]), "spatial")
+        space.add_subspace("stages", KnobSpace("stages", [0, 2, 3, 4]), "reduce")
+        splits = [0, 1, 2, 4, 8] if op.kind == "linear" else [0]
+        space.add_subspace("split_k", KnobSpace("split_k", splits), "reduce")
     else:  # depthwise
         out_h = extents["h"]
         strips = sorted(set(_divisor_like(out_h, [1, 2, 4, 7, 8, 14, 16, 28, 32, 56, 64, 112]) + [out_h]))

@@ -18,10 +18,12 @@ from .configs.grouped_config import grouped_shapes, dilation_shapes
 from .configs.conv1d_config import conv1d_shapes
 from .configs.conv3d_config import conv3d_shapes
 from .configs.gemm_config import gemm_shapes, test_gemm_shapes, b200_batch_gemm_shapes, b200_gemm_int8_shapes
+from .configs.linear_config import linear_shapes, expert_shapes
 from .ir import placeholder
 from .nn import conv2d_nchw, depthwise_conv2d_nchw, gemm as op_gemm, batch_gemm as op_batch_gemm, \
     gemm_int8 as op_gemm_int8, conv1d as op_conv1d, gemm_conv2d_nchw, conv2d_1x1_packed as op_1x1_packed, conv3d_ncdhw, \
-    conv2d_nhwc
+    conv2d_nhwc, linear as op_linear, route_experts as op_route_experts, expert_plan as op_expert_plan, \
+    expert_linear as op_expert_linear, expert_combine as op_expert_combine
 from .space import EnumSpace
 
 TASK_TABLE = {}
@@ -130,6 +132,29 @@ def gemm_int8(N, K, M, transposeB=False):
     return [Output.op], [A, B, Output]
 
 
+def linear(T, N, K, activation="none", gated=False, bias=True, residual=True, dtype="bfloat16"):
+    """act(x . W^T + b) + r on T tokens (gated: both halves of W), one kernel."""
+    wide = 2 * N if gated else N
+    X, W = placeholder((T, K), dtype=dtype), placeholder((wide, K), dtype=dtype)
+    Bias = placeholder((wide,), dtype=dtype) if bias else None
+    R = placeholder((T, N), dtype=dtype) if residual else None
+    Output = op_linear(X, W, bias=Bias, residual=R, activation=activation, gated=gated)
+    return [Output.op], [t for t in (X, W, Bias, R) if t is not None] + [Output]
+
+
+def expert_ffn(T, E, top_k, D, H, activation="silu", scoring="softmax", dtype="bfloat16"):
+    """A routed feed-forward block: the experts of T tokens from their logits, the gated product of every expert's rows,
+    the product back and the weighted sum per token.  Every intermediate is one of the buffers."""
+    X, Logits = placeholder((T, D), dtype=dtype), placeholder((T, E))
+    W1, W2 = placeholder((E, 2 * H, D), dtype=dtype), placeholder((E, D, H), dtype=dtype)
+    Ids, Weights = op_route_experts(Logits, top_k, scoring=scoring)
+    Plan = op_expert_plan(Ids, E)
+    Hidden = op_expert_linear(X, W1, Plan, activation=activation, gated=True, gather=True)
+    Y = op_expert_linear(Hidden, W2, Plan)
+    Output = op_expert_combine(Y, Plan, weights=Weights, residual=X)
+    return [Output.op], [X, Logits, W1, W2, Ids, Weights] + list(Plan) + [Hidden, Y, Output]
+
+
 # ---------------------------------------------------------------- registrations
 def _register_all(category, name, func, args, targets=("llvm", "cuda")):
     for dev in range(NUM_DEVICES):
@@ -194,3 +219,9 @@ for _shape in list(test_gemm_shapes) + list(b200_batch_gemm_shapes):
 
 for _shape in b200_gemm_int8_shapes:
     _register_all("gemm", "gemm_int8", gemm_int8, tuple(_shape))
+
+for _shape in linear_shapes:
+    _register_all("linear", "linear", linear, tuple(_shape))
+
+for _shape in expert_shapes:
+    _register_all("experts", "expert_ffn", expert_ffn, tuple(_shape))

@@ -810,7 +810,7 @@ class Block(object):
         dx, = torch.autograd.grad((routed * self.dout.double()).sum(), x, retain_graph=True)
         out = self.x.double() + gate(self.x.double() @ s1.T) @ s2.T + routed
         g = torch.autograd.grad((out * self.dout.double()).sum(), [w1, w2, s1, s2, logits])
-        return [out, w, g[0], g[1], g[2], g[3], dx, g[4]]
+        return [v.detach() for v in (out, w)] + [g[0], g[1], g[2], g[3], dx, g[4]]
 
     def check(self):
         self.B.check_status(self.status)
@@ -893,3 +893,69 @@ def test_streams_are_named(B):
     B.linear(late, w, out, stream=side)
     side.synchronize()
     assert torch.equal(out, want)
+
+
+# ---------------------------------------------------------------- the same through tasks and modules
+def test_linear_task(B):
+    from flextensor_b200.runtime import build
+    from flextensor_b200.scheduler import schedule_with_config
+    from flextensor_b200.utils import Config
+    key = "linear_linear_(64, 4096, 4096, 'gelu', False)_cuda(0)"
+    x, w, b, r = rand(1, 64, 4096), rand(2, 4096, 4096, scale=1 / 64), rand(3, 4096), rand(4, 64, 4096)
+    want, tol, _, _ = forward64(x, w, b, r, "gelu", False)
+    for config in ({}, {"spatial": [[32], [1]], "reduce": [[2], [4]]}, {"spatial": [[128], [2]], "reduce": [[0], [0]]}):
+        s, bufs = schedule_with_config(key, Config([config], None))
+        func = build(s, bufs, "cuda")
+        out = torch.full((64, 4096), float("nan"), device="cuda", dtype=torch.bfloat16)
+        func(x, w, b, r, out)
+        func.check()
+        bounded(out, want, tol + store(want, torch.bfloat16), str(config))
+    assert func.time_evaluator(func.entry_name, None, number=3)(x, w, b, r, out).mean < 1e-2
+
+
+def test_linear_search(B):
+    from flextensor_b200 import scheduler as S
+    from flextensor_b200.measure import InProcessMeasurer
+    import numpy as np
+    S.VERBOSE = False
+    np.random.seed(0)
+    torch.manual_seed(0)
+    key = "linear_linear_(64, 4096, 4096, 'gelu', False)_cuda(0)"
+    plan, bufs, configs = S.schedule(key, op_trial=3, op_stop=2, timeout=10, parallel=1, number=3, measurer=InProcessMeasurer(0))
+    x, w, b, r = rand(1, 64, 4096), rand(2, 4096, 4096, scale=1 / 64), rand(3, 4096), rand(4, 64, 4096)
+    out = torch.empty(64, 4096, device="cuda", dtype=torch.bfloat16)
+    plan.build()(x, w, b, r, out)
+    want, tol, _, _ = forward64(x, w, b, r, "gelu", False)
+    bounded(out, want, tol + store(want, torch.bfloat16), "found")
+
+
+def test_expert_ffn_task_captured(B):
+    from flextensor_b200.runtime import build
+    from flextensor_b200.scheduler import schedule_with_config
+    from flextensor_b200.utils import Config
+    t, e, k, d, h = 8, 64, 8, 2048, 1024
+    s, bufs = schedule_with_config("experts_expert_ffn_(8, 64, 8, 2048, 1024)_cuda(0)", Config([], None))
+    func = build(s, bufs, "cuda")
+    from flextensor_b200.runtime import torch_dtype
+    arrays = [torch.zeros(tuple(int(v) for v in b.shape), device="cuda", dtype=torch_dtype(b.dtype)) for b in bufs]
+    x, logits, w1, w2 = arrays[:4]
+    w1.copy_(rand(3, e, 2 * h, d, scale=d ** -0.5))
+    w2.copy_(rand(4, e, d, h, scale=h ** -0.5))
+    call = func.capture(*arrays)
+    for seed in (10, 20):
+        x.copy_(rand(seed, t, d))
+        logits.copy_(rand(seed + 1, t, e, dtype=torch.float32))
+        call.replay()
+        torch.cuda.synchronize()
+        func.check()
+        ids, weights = route64(logits, k, None, "softmax", 1, 1, True, 1.0)
+        assert torch.equal(arrays[4], ids)
+        want = x.double()
+        for i in range(e):
+            mine = weights * (ids == i)
+            rows = mine.sum(1) > 0
+            if rows.any():
+                z = x[rows].double() @ w1[i].double().T
+                want[rows] += mine[rows].sum(1, keepdim=True) * ((act64(z[:, :h], "silu") * z[:, h:]) @ w2[i].double().T)
+        # three stores on the way (hidden, y, out), the first two scaled by weights of at most one
+        assert float((arrays[-1].double() - want).abs().max()) <= 8 * 3 * 2.0 ** -8 * float(want.square().mean().sqrt() + 1)
