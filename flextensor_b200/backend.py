@@ -601,21 +601,25 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 SCORINGS = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
+_ELEMENTS = (torch.bfloat16, torch.float16)
 
 
 def _element(t, name):
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float16) or not t.is_cuda:
+    dtype = getattr(t, "dtype", None)
+    if dtype not in _ELEMENTS or not t.is_cuda:
         raise TypeError("%s must be a bfloat16 or float16 CUDA tensor" % name)
-    return t.dtype
+    return dtype
 
 
 def _fits(t, name, shape, dtype, device):
     """One operand's type, device, layout and shape; its address (None passes through)."""
     if t is None:
         return None
-    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.shape == shape and
-            t.is_contiguous()):
-        return t.data_ptr()
+    try:  # what a fitting tensor answers; anything else is named below
+        if t.dtype is dtype and t.get_device() == device.index and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA tensor" % name)
     if t.dtype != dtype:
@@ -662,14 +666,15 @@ def _status_of(status, device):
 
 
 def _logits(t):
-    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES or not t.is_cuda:
+    if getattr(t, "dtype", None) not in DTYPES or not t.is_cuda:
         raise TypeError("logits must be a float32, bfloat16 or float16 CUDA tensor")
 
 
 def _matrix(t, name, dims):
-    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+    shape = getattr(t, "shape", ())
+    if len(shape) != dims:
         raise ValueError("%s must have %d dimensions" % (name, dims))
-    return t.shape
+    return shape
 
 
 def linear(x, weight, out, bias=None, residual=None, activation="none", gated=False, preact=None, cfg=None, status=None,

@@ -56,6 +56,7 @@ struct LinUmma {
   LinArgs q;
   int bn, bj;            // tokens per tile, and of those staged per CTA
   int stages, split;
+  int most_rows;         // LIN_ROWS: token tiles of a plan, at most (offsets that are none cannot ask for more)
   int tiles_i, tiles_j;  // tiles_j: LIN_DENSE and LIN_REDUCE
   int feat, sub_off;     // features per tile; feature rows between the A sub-tiles
   int band;              // token tiles walked together before the next feature tile
@@ -321,6 +322,9 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
     prefetch_tmap(&maps.a);
     prefetch_tmap(&maps.b);
   }
+  // The kernel before this one may still run and may not hold all the tensor memory yet that it is going to need: this
+  // one asks for its own only after it.
+  grid_dependency_wait();
   if (warp == 1) {
     if constexpr (PAIR) {
       tmem_alloc_pair(smem_u32(&tmem_slot), p.tmem_cols);
@@ -331,7 +335,6 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
     }
   }
   if (warp == 3 && mode == LIN_ROWS) {
-    grid_dependency_wait();
     // token tiles before each group
     int base = 0;
     for (int g0 = 0; g0 < p.q.groups; g0 += 32) {
@@ -347,8 +350,8 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
         const int y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
       }
-      if (g0 + lane < p.q.groups) tstart[g0 + lane + 1] = base + x;
-      base += __shfl_sync(0xffffffffu, x, 31);
+      if (g0 + lane < p.q.groups) tstart[g0 + lane + 1] = min(base + x, p.most_rows);
+      base = min(base + __shfl_sync(0xffffffffu, x, 31), p.most_rows);
     }
     if (lane == 0) tstart[0] = 0;
   }
@@ -358,7 +361,6 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_slot, 0);
   grid_launch_dependents();  // tensor memory is held: a successor's CTA on this SM cannot take it first
-  grid_dependency_wait();
 
   const int total = mode == LIN_ROWS ? tstart[p.q.groups] * p.tiles_i : p.q.groups * p.tiles_i * p.tiles_j;
   const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
@@ -590,7 +592,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
       const long long j0 = static_cast<long long>(c.tj) * p.bn;
       const int left = static_cast<int>(min((mode == LIN_ROWS ? static_cast<long long>(c.cnt) : p.q.J) - j0,
                                             static_cast<long long>(p.bn)));
-      const long long row0 = (mode == LIN_ROWS ? c.lo : 0) + j0;
+      const long long row0 = (mode == LIN_ROWS ? c.lo : 0) + j0;  // (left <= 0: no column is stored)
       const long long out_base = mode == LIN_REDUCE ? c.g * p.q.out_gs : 0;
       constexpr bool GATED = FORM == FORM_GATED;
       const int first = FORM == FORM_WIDE ? 0 : grp * kCols, step = FORM == FORM_WIDE ? kCols : GROUPS * kCols;
@@ -964,6 +966,7 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
   p.sub_off = c.form == FORM_WIDE ? m : static_cast<int>(q.I);
   p.tiles_i = static_cast<int>(ceil_div64(q.I, p.feat));
   p.tiles_j = static_cast<int>(q.mode == LIN_ROWS ? 1 : ceil_div64(q.J, c.bn));
+  p.most_rows = static_cast<int>(most / p.tiles_i);
   p.band = 8;
   p.by_i = fast_div(p.tiles_i);
   p.by_group = fast_div(static_cast<int64_t>(p.tiles_i) * p.tiles_j);

@@ -78,28 +78,7 @@ __device__ __forceinline__ float act_value(float z, int act) {
   }
 }
 
-// act'(z); relu has 0 at 0.
-__device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-    case FTB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-    case FTB_ACT_GELU: {
-      float bell;
-      const float cdf = normal_cdf(z, &bell);
-      return fmaf(z * 0.3989422804014327f, bell, cdf);
-    }
-    case FTB_ACT_GELU_TANH: {
-      const float s = sigmoid_f(2.0f * kGeluC * (z + kGeluA * z * z * z));
-      return s + 2.0f * z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
-    }
-    case FTB_ACT_SILU: {
-      const float s = sigmoid_f(z);
-      return s * (1.0f + z * (1.0f - s));
-    }
-    default: return 1.0f;
-  }
-}
-
-// act(z) and act'(z) of N values: one branch, then straight-line code that shares the exponential.
+// act(z) and act'(z) of N values (relu' is 0 at 0): one branch, then straight-line code that shares the exponential.
 template <int N>
 __device__ __forceinline__ void act_both(const float (&z)[N], float (&value)[N], float (&slope)[N], int act) {
   if (act == FTB_ACT_SILU) {
@@ -142,8 +121,8 @@ __device__ __forceinline__ void act_both(const float (&z)[N], float (&value)[N],
 // ------------------------------------------------------------------ launches that overlap
 // Every kernel of the feed-forward operators is launched as a programmatic dependent: its set-up runs while the kernel
 // before it in the stream drains.  Each waits (griddepcontrol.wait) before its first access to global memory, so what
-// an earlier kernel of any kind wrote is seen, and lets its own successor start only once it holds every resource that
-// it may have to wait for (tensor memory).
+// an earlier kernel of any kind wrote is seen, asks for tensor memory only after that wait, and lets its own successor
+// start only once it holds it: no kernel can take columns that one it waits for still needs.
 template <typename... Params, typename... Args>
 inline int launch_overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream,
                              Args... args) {

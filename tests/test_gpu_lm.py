@@ -742,6 +742,95 @@ def test_expert_large(B, status, gather, gated):
     assert not out[used:].any() and not dx[used:].any()
 
 
+def shifted(t, by=1):
+    """The same values in a contiguous tensor whose base is ``by`` elements off a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 16, device="cuda", dtype=t.dtype)
+    view = flat[by:by + t.numel()].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_unaligned_bases(B, status, which):
+    """Any one operand, or all of them, off a 16-byte boundary: other accesses, the same values within their bounds."""
+    t, n, k = 70, 136, 128
+    x, w, b, r, dy = rand(1, t, k), rand(2, 2 * n, k, scale=0.1), rand(3, 2 * n), rand(4, t, n), rand(5, t, n)
+    move = lambda i, v: shifted(v) if which in (i, 5) else v
+    x, w, r, dy = move(0, x), move(1, w), move(2, r), move(4, dy)
+    out, z = move(3, torch.empty_like(r)), move(4, torch.empty(t, 2 * n, device="cuda", dtype=torch.bfloat16))
+    B.linear(x, w, out, bias=move(2, b), residual=r, activation="silu", gated=True, preact=z, status=status)
+    want, tol, z64, ez = forward64(x, w, b, r, "silu", True)
+    bounded(out, want, tol + store(want, torch.bfloat16), "out")
+    bounded(z, z64, ez + store(z64, torch.bfloat16), "preact")
+    dx, dw, db = move(0, torch.empty_like(x)), move(1, torch.empty_like(w)), move(2, torch.empty_like(b))
+    ws = torch.empty(B.linear_backward_workspace_bytes(t, n, k, True), dtype=torch.uint8, device="cuda")
+    B.linear_backward(x, w, dy, dx=dx, dweight=dw, dbias=db, preact=z, activation="silu", gated=True, workspace=ws, status=status)
+    want = gradients64(x, w, dy, z, "silu", True)
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        bounded(got, *want[name], name)
+    logits = move(0, rand(6, t, 64, dtype=torch.float32))
+    bias = move(1, rand(7, 64, dtype=torch.float32))
+    ids, weights = torch.empty(t, 4, device="cuda", dtype=torch.int32), torch.empty(t, 4, device="cuda")
+    B.route_experts(logits, ids, weights, bias=bias, scoring="sigmoid", groups=4, top_groups=2)
+    assert torch.equal(ids, route64(logits, 4, bias, "sigmoid", 4, 2, True, 1.0)[0])
+    plan = planned(B, ids, 64)
+    y = move(3, rand(8, t * 4, n))
+    got = move(4, torch.empty(t, n, device="cuda", dtype=torch.bfloat16))
+    B.expert_combine(y, plan, got, weights=weights)
+    part = y.double()[plan.slots.long()].view(t, 4, n) * weights.double()[:, :, None]
+    bounded(got, part.sum(1), 10 * E * part.abs().sum(1) + store(part.sum(1), torch.bfloat16), "combine")
+
+
+def test_every_row_dropped(B, status):
+    t, k, e, n, width = 20, 3, 5, 72, 64
+    plan = planned(B, torch.full((t, k), -1, device="cuda", dtype=torch.int32), e)
+    assert plan.offsets.tolist() == [0] * 6 and (plan.order == -1).all() and (plan.slots == -1).all()
+    nan = lambda *s: torch.full(s, float("nan"), device="cuda", dtype=torch.bfloat16)
+    w = rand(1, e, n, width)
+    out, dx = torch.full((t * k, n), 7.0, device="cuda", dtype=torch.bfloat16), torch.full((t * k, width), 7.0, device="cuda", dtype=torch.bfloat16)
+    for gather in (False, True):
+        x = nan(t if gather else t * k, width)
+        B.expert_linear(x, w, plan, out, gather=gather, status=status)
+        dw, db = nan(e, n, width), nan(e, n)
+        ws = torch.empty(B.expert_linear_backward_workspace_bytes(plan, n, width), dtype=torch.uint8, device="cuda")
+        B.expert_linear_backward(x, w, plan, nan(t * k, n), dx=dx, dweight=dw, dbias=db, gather=gather, workspace=ws, status=status)
+        assert not dw.any() and not db.any()
+    assert (out == 7).all() and (dx == 7).all()
+    r = rand(2, t, n)
+    total, dweights = nan(t, n), torch.full((t, k), float("nan"), device="cuda")
+    B.expert_combine(nan(t * k, n), plan, total, weights=torch.rand(t, k, device="cuda"), residual=r)
+    assert torch.equal(total, r)
+    B.expert_combine_backward(r, plan, y=nan(t * k, n), dweights=dweights)
+    assert not dweights.any()
+
+
+def test_results_past_32_bits(B, status):
+    """An output of 2.3e9 elements: the last rows lie behind 2^31 of them."""
+    t, n, k = 70000, 33000, 64
+    x, w = rand(1, t, k), rand(2, n, k, scale=0.1)
+    out = torch.empty(t, n, device="cuda", dtype=torch.bfloat16)
+    B.linear(x, w, out, activation="relu", status=status)
+    rows = [0, 1, 65000, 65077, t - 2, t - 1]  # 2^31 / 33000 = 65075.3
+    want, tol, _, _ = forward64(x[rows], w, None, None, "relu", False)
+    bounded(out[rows], want, tol + store(want, torch.bfloat16), "rows")
+    del out
+    # the same behind the sorted places of two experts
+    plan = planned(B, (torch.arange(t, device="cuda") >= 40000).to(torch.int32)[:, None].contiguous(), 2)
+    w2 = rand(3, 2, n, k, scale=0.1)
+    out = torch.empty(t, n, device="cuda", dtype=torch.bfloat16)
+    B.expert_linear(x, w2, plan, out, status=status)
+    for i, one in ((0, [0, 39999]), (1, [40000, 65077, t - 1])):
+        want, tol, _, _ = forward64(x[one], w2[i], None, None, "none", False)
+        bounded(out[one], want, tol + store(want, torch.bfloat16), "expert %d" % i)
+    dx = torch.empty_like(x)
+    ws = torch.empty(B.expert_linear_backward_workspace_bytes(plan, n, k), dtype=torch.uint8, device="cuda")
+    B.expert_linear_backward(x, w2, plan, out, dx=dx, workspace=ws, status=status)
+    for i, one in ((0, [0, 39999]), (1, [40000, 65077, t - 1])):
+        dy = out[one].double()
+        want = dy @ w2[i].double()
+        bounded(dx[one], want, 2 * (n + 2) * E * (dy.abs() @ w2[i].double().abs()) + store(want, torch.bfloat16), "dx")
+
+
 # ---------------------------------------------------------------- together, as a model uses them
 class Block(object):
     """A mixture-of-experts feed-forward block with a shared expert, forward and backward, on buffers of its own."""
