@@ -7,8 +7,11 @@
 //   warp 0      producer: TMA tiles of A and B into 128-byte swizzled stages of 64 k; rows named by a list (tokens of
 //               an expert, or the reduction of its weight gradient) come by gather4, four rows per lane and copy, and a
 //               row past the end of its expert is asked for outside the tensor, which fills it with zeros
-//   warp 1, 2   issuers of tcgen05.mma, one per A sub-tile (one thread issues an MMA every 137 cycles at best)
-//   warps 4..   epilogue: tcgen05.ld -> bias, activation, gate, residual -> 2-byte stores, 64 bytes per warp
+//   warp 1, 2   issuers of tcgen05.mma, one per A sub-tile.  The whole warp runs the loop and one elected lane issues:
+//               addresses and descriptors then stay in uniform registers.  Run by a single lane, a stage of four MMAs
+//               took about 900 cycles whatever its tile, now 500 in a pair and 420 alone (256 x 4096 x 4096: 31.4 -> 20.9 us)
+//   warp 3      second loader where rows are fetched by number (a gather4 costs its loader about 50 ns)
+//   warps 4..   epilogue: tcgen05.ld -> bias, activation, gate, residual -> stores
 //
 // Forms: FORM_PLAIN one A sub-tile; FORM_GATED two, the gate rows and the others of the same features, whose
 // accumulators share lanes and columns, so the gate is applied in registers; FORM_WIDE two neighbouring feature tiles
@@ -19,6 +22,18 @@
 //
 // Waits are bounded as in ftb_umma_kernel.cuh: a role that gives up sets a status bit and the CTA leaves through its
 // normal teardown.
+//
+// What bounds it, measured on a B200 (bf16, device time in a CUDA graph of calls on rotating operands):
+//   4096 x 4096 x 4096            95 us   1447 TFLOP/s, 0.89 of the measured matrix rate; rows through the SM's port (256 a
+//                                         stage for 512 cycles of math) and the power cap
+//   8192 x (2 x 8192) x 4096 gated 812 us 1354 TFLOP/s, 0.97 of the sustained rate: the power cap
+//   1 x 4096 x 4096               9.0 us  3.7 TB/s: 5.1 us of reading W, then launch, first copies and the exchange of the
+//                                         partial sums; eight CTAs per tile (four: 9.4, two: 13.5, one: 19.7)
+//   48 x (2 x 8192) x 2048 gated  16.6 us 4.0 TB/s: 10.4 us of reading W
+//   1237 x 2048 x 1000            10.4 us, with GELU, bias, residual and preact 15.2: one wave of tiles whose epilogue
+//                                         nothing covers; 2051 columns, stored in 2-byte accesses: 20.4
+//   16384 places of 32 experts x 2048 x 2048  122 us  1.06 PFLOP/s of useful work: a quarter of the tiles' rows are the ends
+//                                         of groups; the same rows gathered by number 167 us (12 cycles a row)
 #include "ftb_linear.h"
 #include "ftb_ptx.cuh"
 #include "ftb_tmap.h"
