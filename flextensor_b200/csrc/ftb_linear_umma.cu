@@ -325,7 +325,9 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < stages; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 1);
+      // Where the second loader has copies in some blocks only (the last of a reduction) it reports every block, so that
+      // the ring never gets a turn ahead of it and its waits always mean the turn they ask about.
+      mbar_init(smem_u32(&bar_full[s]), 1 + (mode == LIN_REDUCE ? (PAIR ? 2 : 1) : 0));
       mbar_init(smem_u32(&bar_empty[s]), SUBS);
     }
     for (int a = 0; a < 2; ++a) {
@@ -335,7 +337,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
     fence_mbar_init();
     fence_proxy_async_smem();
     prefetch_tmap(&maps.a);
-    prefetch_tmap(&maps.b);
+    prefetch_tmap(mode == LIN_ROWS && p.q.gather_div != 0 ? &maps.b_rows : &maps.b);
   }
   // The kernel before this one may still run and may not hold all the tensor memory yet that it is going to need: this
   // one asks for its own only after it.
@@ -417,8 +419,7 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
         __syncwarp();
       }
       for (int kb = kb0; kb < kb1; ++kb) {
-        const bool tail = gather_k && (kb + 1) * kKBlock > c.cnt;   // the block ends past the group
-        
+        const bool tail = gather_k && (kb + 1) * kKBlock > c.cnt;  // the block ends past the group
         // The last block of a group: whole runs of 16 places as tiles (an MMA takes 16), the places of the run in which
         // the group ends by number, those past it outside the tensors.
         const int runs = tail ? (c.cnt - kb * kKBlock) >> 4 : 0, odd = tail ? (c.cnt - kb * kKBlock) & 15 : 0;
@@ -496,6 +497,10 @@ linear_umma_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
                 else tma_gather4(at, m1, full, col, r0, r1, r2, r3);
               }
             }
+          }
+          if (gather_k && part == 1) {
+            if constexpr (PAIR) mbar_arrive_cluster(full);
+            else mbar_arrive(full);
           }
         }
         __syncwarp();
@@ -790,7 +795,7 @@ struct LinPick {
   bool pair;
   int form, bn, split;
   bool deep;  // single CTAs with an SM's shared memory each: no more of them than SMs, and clusters of at most four
-              // (eight such CTAs find room in a GPC twice at best: 22 us against 16 with four, 8 x 2048 x 8192)
+              // (eight such CTAs find room in a GPC twice at best: 22 us for 8 x 2048 x 8192, 10 with two CTAs an SM)
 };
 
 static size_t stage_size(const LinPick& c) {
