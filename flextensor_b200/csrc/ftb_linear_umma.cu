@@ -191,6 +191,12 @@ __device__ __forceinline__ void lin_residual(bool vec, const WarpCols& w, uint32
       res[4 * h + 2] = x.z;
       res[4 * h + 3] = x.w;
     }
+  } else if (w.live && w.valid >= kCols) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      res[c] = *r;
+      r += pitch;
+    }
   } else {
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
@@ -226,13 +232,22 @@ __device__ __forceinline__ void lin_store(bool vec, bool f16, const WarpCols& w,
         *reinterpret_cast<uint4*>(o + (h ? 8 * pitch : 0)) =
             make_uint4(pack16(x[0], x[1], f16), pack16(x[2], x[3], f16), pack16(x[4], x[5], f16), pack16(x[6], x[7], f16));
     }
-  } else {
+  } else if (w.live) {
+    float x[kCols];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      float x = v[c];
-      if (res) x += from16(static_cast<uint16_t>(res[c]), f16);
-      if (w.live && c < w.valid) *o = to16(x, f16);
-      o += pitch;
+    for (int c = 0; c < kCols; ++c) x[c] = res ? v[c] + from16(static_cast<uint16_t>(res[c]), f16) : v[c];
+    if (w.valid >= kCols) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        *o = to16(x[c], f16);
+        o += pitch;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        if (c < w.valid) *o = to16(x[c], f16);
+        o += pitch;
+      }
     }
   }
 }
