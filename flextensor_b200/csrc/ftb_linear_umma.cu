@@ -27,11 +27,11 @@
 //   4096 x 4096 x 4096            95 us   1447 TFLOP/s, 0.89 of the measured matrix rate; rows through the SM's port (256 a
 //                                         stage for 512 cycles of math) and the power cap
 //   8192 x (2 x 8192) x 4096 gated 812 us 1354 TFLOP/s, 0.97 of the sustained rate: the power cap
-//   1 x 4096 x 4096               9.0 us  3.7 TB/s: 5.1 us of reading W, then launch, first copies and the exchange of the
+//   1 x 4096 x 4096               9.3 us  3.6 TB/s: 5.1 us of reading W, then launch, first copies and the exchange of the
 //                                         partial sums; eight CTAs per tile (four: 9.4, two: 13.5, one: 19.7)
 //   48 x (2 x 8192) x 2048 gated  16.6 us 4.0 TB/s: 10.4 us of reading W
-//   1237 x 2048 x 1000            10.4 us, with GELU, bias, residual and preact 15.2: one wave of tiles whose epilogue
-//                                         nothing covers; 2051 columns, stored in 2-byte accesses: 20.4
+//   1237 x 2048 x 1000            10.9 us, with GELU, bias, residual and preact 15.8: one wave of tiles whose epilogue
+//                                         nothing covers; 2051 columns, stored in 2-byte accesses: 16.4
 //   16384 places of 32 experts x 2048 x 2048  122 us  1.06 PFLOP/s of useful work: a quarter of the tiles' rows are the ends
 //                                         of groups; the same rows gathered by number 167 us (12 cycles a row)
 #include "ftb_linear.h"
@@ -162,9 +162,8 @@ __device__ __forceinline__ void act_values(float (&v)[NC], int act) {
 // The epilogue of 16 columns (tokens) by one warp, whose lanes hold 32 neighbouring features.  The arithmetic runs as
 // the accumulator lies, a feature per lane.  Where every row of the results starts on 16 bytes (`vec`) a warp then turns
 // its 16 x 32 values round through 2.25 KB of shared memory and a lane loads and stores eight features of a token at a
-// time: about a quarter of the instructions of 2-byte accesses, which bound the epilogue (GELU with bias, residual and
-// preact at 1237 x 2051 x 1000: 10 us of 21 before).  Rows of other pitches keep the 2-byte accesses, 64 contiguous
-// bytes per warp.
+// time.  Rows of other pitches keep 2-byte accesses, 64 contiguous bytes per warp, without predicates where all columns
+// are tokens (GELU with bias, residual and preact, 1237 x 2048 x 1000: 15.8 us; 2051 columns: 16.4, with predicates 21.2).
 constexpr int kCols = 16;          // columns a thread holds at a time
 constexpr int kTurnPitch = 36;     // floats between two tokens: a lane's 16-byte reads meet no bank twice
 constexpr int kTurnFloats = kCols * kTurnPitch;

@@ -968,6 +968,44 @@ def test_block_on_another_stream(B):
         block.check()
 
 
+def test_graph_with_branches(B):
+    """Two products on forked streams, a copy and a third product behind the join, captured and replayed."""
+    x, w = rand(1, 40, 256), [rand(i, 256, 256, scale=1 / 16) for i in (2, 3, 4)]
+    new = lambda: torch.zeros(40, 256, device="cuda", dtype=torch.bfloat16)
+    a, b, c, out = new(), new(), new(), new()
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        B.linear(x, w[0], a, activation="silu")
+        with torch.cuda.stream(side):
+            B.linear(x, w[1], b, activation="relu")
+        main.wait_stream(side)
+        c.copy_(a)
+        c.add_(b)
+        B.linear(c, w[2], out, residual=b)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed in (7, 8):
+        x.copy_(rand(seed, 40, 256))
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (a, b, out)]
+        for t in (a, b, c, out):
+            t.fill_(float("nan"))
+        run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, t) for g, t in zip(got, (a, b, out)))
+        want, tol, _, _ = forward64(c, w[2], None, b, "none", False)
+        bounded(out, want, tol + store(want, torch.bfloat16), "out")
+
+
 def test_streams_are_named(B):
     """The ``stream`` argument: the call runs behind that stream's work, not the current one's."""
     x, w = rand(1, 64, 128), rand(2, 96, 128, scale=0.1)
