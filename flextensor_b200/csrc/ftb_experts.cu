@@ -10,15 +10,27 @@ namespace cg = cooperative_groups;
 
 // ------------------------------------------------------------------ stable counting sort of expert ids
 // One cluster does it in one launch: a CTA owns a run of rows, a warp a run of the CTA's.  Every warp counts its ids
-// into a row of shared memory of its own (lanes with equal ids find each other with a match, so nothing is added
+// into a row of shared memory of its own (lanes with equal ids find each other by ballots, so nothing is added
 // atomically and the result does not depend on timing), the counts are summed over warps, over the CTAs of the cluster
-// (through distributed shared memory) and over the experts, and the warps walk their rows a second time to hand out
-// places.  Bytes: ids twice (the second time from L2), order and slots once; bound by latency: 3.7 us for 4000 rows of 16
-// experts, 7.1 us for 16384 rows of 32 (device time, in a graph).
+// (through distributed shared memory) and over the experts, and a second walk gives every row its place.  Bytes: ids
+// twice (the second time from L2), order once, slots three times; bound by latency up to some ten thousand rows (device time,
+// in a graph: 64 rows of 64 experts 2.6 us, 4000 of 16 3.4, 16384 of 32 5.7, 32768 of 256 10.2), then by the scattered
+// stores of eight SMs (262144 rows of 256: 49 us, beside products of milliseconds).
 constexpr int kPlanCtas = 8;
 
+// Lanes with the same key (`bits` of it): one ballot per bit.
+__device__ __forceinline__ unsigned same_key(int key, int bits) {
+  unsigned same = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (key >> b) & 1;
+    const unsigned ones = __ballot_sync(0xffffffffu, one);
+    same &= one ? ones : ~ones;
+  }
+  return same;
+}
+
 __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict__ ids, int* __restrict__ offsets,
-                                                           int* __restrict__ order, int* __restrict__ slots, int rows,
+                                                           int* __restrict__ order, int* slots, int rows,
                                                            int experts) {
   extern __shared__ int smem[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -31,16 +43,27 @@ __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict
   const long long per_warp = ((static_cast<long long>(rows) + ctas * warps - 1) / (ctas * warps) + 31) / 32 * 32;
   const long long r0 = (static_cast<long long>(rank) * warps + warp) * per_warp;
   const long long r1 = min(r0 + per_warp, static_cast<long long>(rows));
+  const int bits = 32 - __clz(experts);  // of keys 0..experts, the last standing for dropped rows
   int* mine = hist + warp * experts;
   for (int e = lane; e < experts; e += 32) mine[e] = 0;
   __syncwarp();
   grid_dependency_wait();
   grid_launch_dependents();
+  auto id_of = [&](long long row) {
+    const int key = row < r1 ? ids[row] : experts;
+    return key < 0 || key > experts ? experts : key;
+  };
+  // A row's number among its warp's rows of the same expert waits in `slots` for the second walk, which then has no
+  // order to keep; the next ids are on their way meanwhile.
+  int next = id_of(r0 + lane);
   for (long long r = r0; r < r1; r += 32) {
-    int key = r + lane < r1 ? ids[r + lane] : -1;
-    if (key >= experts) key = -1;
-    const unsigned same = __match_any_sync(0xffffffffu, key < 0 ? -1 : key);
-    if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
+    const int key = next;
+    next = id_of(r + 32 + lane);
+    const unsigned same = same_key(key, bits);
+    const int before = key < experts ? mine[key] : 0;
+    if (r + lane < r1) slots[r + lane] = before + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (key < experts && lane == __ffs(same) - 1) mine[key] = before + __popc(same);
     __syncwarp();
   }
   __syncthreads();
@@ -56,11 +79,13 @@ __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict
   cluster.sync();
   // counts of all CTAs, and of those before this one
   for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-    int before = 0, all = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const int v = cluster.map_shared_rank(total, c)[e];
-      if (c < rank) before += v;
-      all += v;
+    int before = 0, all = 0, v[kPlanCtas];
+#pragma unroll
+    for (int c = 0; c < kPlanCtas; ++c) v[c] = c < ctas ? cluster.map_shared_rank(total, c)[e] : 0;
+#pragma unroll
+    for (int c = 0; c < kPlanCtas; ++c) {
+      if (c < rank) before += v[c];
+      all += v[c];
     }
     start[e] = before;
     // the total over CTAs goes where the warps' scan below finds it; own total is not needed any more once every CTA
@@ -91,19 +116,12 @@ __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict
     }
   }
   __syncthreads();
-  for (long long r = r0; r < r1; r += 32) {
-    int key = r + lane < r1 ? ids[r + lane] : -1;
-    if (key >= experts) key = -1;
-    const unsigned same = __match_any_sync(0xffffffffu, key < 0 ? -1 : key);
-    int place = -1;
-    if (key >= 0) place = start[key] + mine[key] + __popc(same & ((1u << lane) - 1u));
-    __syncwarp();
-    if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
-    __syncwarp();
-    if (r + lane < r1) {
-      slots[r + lane] = place;
-      if (place >= 0) order[place] = static_cast<int>(r) + lane;
-    }
+#pragma unroll 4
+  for (long long row = r0 + lane; row < r1; row += 32) {
+    const int key = id_of(row);
+    const int place = key < experts ? start[key] + mine[key] + slots[row] : -1;
+    slots[row] = place;
+    if (place >= 0) order[place] = static_cast<int>(row);
   }
   for (long long q = placed + static_cast<long long>(rank) * blockDim.x + threadIdx.x; q < rows;
        q += static_cast<long long>(ctas) * blockDim.x)
@@ -112,7 +130,7 @@ __global__ void __launch_bounds__(1024) expert_plan_kernel(const int* __restrict
 
 static int launch_plan(const int* ids, int* offsets, int* order, int* slots, int64_t rows, int64_t experts,
                        cudaStream_t stream) {
-  // one CTA up to 1024 rows (32 rows a warp); above that eight share them (4000 rows: 3.7 us against 10.3 in one)
+  // one CTA up to 1024 rows (32 rows a warp); above that eight share them (4000 rows: 3.4 us, in one 10.3)
   const int ctas = rows > 1024 ? kPlanCtas : 1;
   int64_t warps = ceil_div64(rows, static_cast<int64_t>(ctas) * 32);
   if (warps < 4) warps = 4;
@@ -137,7 +155,7 @@ static int launch_plan(const int* ids, int* offsets, int* order, int* slots, int
 
 // ------------------------------------------------------------------ weighted sum of a token's rows
 // Bound by reading y once; a thread owns VEC neighbouring columns of one token and adds its rows in slot order in fp32.
-// 4096 tokens x 4 rows x 2048 with residual: 19.8 us, 5.1 TB/s, 0.78 of the measured copy rate.
+// 4096 tokens x 4 rows x 2048 with residual: 17.6 us, 5.7 TB/s, 0.87 of the measured copy rate.
 template <int VEC>
 __global__ void __launch_bounds__(128)
 expert_combine_kernel(const uint16_t* __restrict__ y, const int* __restrict__ slots, const float* __restrict__ weights,
@@ -164,23 +182,36 @@ expert_combine_kernel(const uint16_t* __restrict__ y, const int* __restrict__ sl
       acc[0] = from16(residual[t * n + c], f16);
     }
   }
+  // four rows on their way at a time, added in slot order
   const int* slot = slots + t * top_k;
-#pragma unroll 4
-  for (int j = 0; j < top_k; ++j) {
-    const int place = slot[j];
-    if (place < 0 || place >= rows) continue;
-    const float w = weights ? weights[t * top_k + j] : 1.0f;
-    if constexpr (VEC == 8) {
-      const uint4 q = *reinterpret_cast<const uint4*>(y + place * n + c);
-      const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+  for (int j0 = 0; j0 < top_k; j0 += 4) {
+    float w[4];
+    uint4 q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack16(v[i], f16);
-        acc[2 * i] = fmaf(w, f.x, acc[2 * i]);
-        acc[2 * i + 1] = fmaf(w, f.y, acc[2 * i + 1]);
+    for (int e = 0; e < 4; ++e) {
+      const int place = j0 + e < top_k ? slot[j0 + e] : -1;
+      const bool there = place >= 0 && place < rows;
+      w[e] = !there ? 0.0f : weights ? weights[t * top_k + j0 + e] : 1.0f;
+      q[e] = make_uint4(0, 0, 0, 0);
+      if constexpr (VEC == 8) {
+        if (there) q[e] = *reinterpret_cast<const uint4*>(y + place * n + c);
+      } else {
+        if (there) q[e].x = y[place * n + c];
       }
-    } else {
-      acc[0] = fmaf(w, from16(y[place * n + c], f16), acc[0]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (VEC == 8) {
+        const uint32_t v[4] = {q[e].x, q[e].y, q[e].z, q[e].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack16(v[i], f16);
+          acc[2 * i] = fmaf(w[e], f.x, acc[2 * i]);
+          acc[2 * i + 1] = fmaf(w[e], f.y, acc[2 * i + 1]);
+        }
+      } else {
+        acc[0] = fmaf(w[e], from16(static_cast<uint16_t>(q[e].x), f16), acc[0]);
+      }
     }
   }
   if constexpr (VEC == 8) {
