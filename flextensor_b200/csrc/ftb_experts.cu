@@ -323,8 +323,8 @@ int ftb_expert_combine_backward(int dtype, const void* dout, const void* y, cons
   using namespace ftb;
   int rc = combine_checks(dtype, tokens, top_k, n);
   if (rc) return rc;
-  if (!dy && !dweights) return FTB_E_BAD_ARG;
   if (tokens == 0) return FTB_OK;
+  if (!dy && !dweights) return FTB_E_BAD_ARG;
   if (!dout || !slots || (dweights && !y)) return FTB_E_BAD_ARG;
   rc = device_ok();
   if (rc) return rc;

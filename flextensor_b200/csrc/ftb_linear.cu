@@ -366,7 +366,7 @@ int ftb_linear_backward(int dtype, const void* x, const void* w, const void* dy,
   using namespace ftb;
   const int rc = check_common(dtype, tokens, n, k, activation, gated);
   if (rc) return rc;
-  if (!dx && !dw && !db) return FTB_E_BAD_ARG;
+  if (!dx && !dw && !db) return tokens == 0 ? FTB_OK : FTB_E_BAD_ARG;  // (an empty dx has no address)
   return backward_generic(dtype, x, w, nullptr, nullptr, dy, preact, dx, dw, db, tokens, tokens, 1, n, k, activation,
                           gated, 0, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
@@ -434,7 +434,8 @@ int ftb_expert_linear_backward(int dtype, const void* x, const void* w, const in
   int rc = check_common(dtype, rows, n, k, activation, gated);
   if (!rc) rc = check_experts(rows, top_k, experts);
   if (rc) return rc;
-  if (gather < 0 || gather > 1 || !offsets || (gather && !order) || (!dx && !dw && !db)) return FTB_E_BAD_ARG;
+  if (gather < 0 || gather > 1 || !offsets || (rows > 0 && gather && !order)) return FTB_E_BAD_ARG;
+  if (!dx && !dw && !db) return rows == 0 ? FTB_OK : FTB_E_BAD_ARG;
   return backward_generic(dtype, x, w, offsets, order, dy, preact, dx, dw, db, rows, gather ? rows / top_k : rows, experts,
                           n, k, activation, gated, gather ? static_cast<int>(top_k) : 0, workspace, workspace_bytes,
                           status, static_cast<cudaStream_t>(stream));

@@ -494,7 +494,7 @@ def test_expert_plan_empty(B):
 
 
 EXPERTS = [(1, 1, 1, 64, 64), (1, 8, 64, 130, 128), (3, 2, 4, 7, 8), (16, 4, 8, 256, 200), (100, 2, 5, 300, 136),
-           (257, 3, 6, 129, 64), (40, 6, 128, 64, 72), (600, 2, 3, 512, 264), (50, 2, 4, 33, 20), (2000, 1, 9, 96, 96)]
+           (257, 3, 6, 129, 64), (40, 6, 128, 64, 72), (600, 2, 3, 512, 264), (50, 2, 4, 33, 20), (2000, 1, 9, 96, 96), (3, 32, 1024, 40, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -802,6 +802,45 @@ def test_every_row_dropped(B, status):
     assert torch.equal(total, r)
     B.expert_combine_backward(r, plan, y=nan(t * k, n), dweights=dweights)
     assert not dweights.any()
+
+
+def test_no_tokens_anywhere(B):
+    new = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, device="cuda", dtype=dtype)
+    logits, ids, weights = new(0, 8, dtype=torch.float32), new(0, 2, dtype=torch.int32), new(0, 2, dtype=torch.float32)
+    B.route_experts(logits, ids, weights, groups=2, top_groups=1)
+    B.route_experts_backward(logits, ids, weights, logits)
+    plan = planned(B, ids, 8)
+    y, out = new(0, 24), new(0, 24)
+    B.expert_combine(y, plan, out, weights=weights)
+    B.expert_combine_backward(out, plan, y=y, dy=y, dweights=weights)
+    assert plan.offsets.tolist() == [0] * 9
+    w = rand(1, 8, 24, 16)
+    ws = torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    for gather in (False, True):
+        dw, db = torch.ones_like(w), torch.ones(8, 24, device="cuda", dtype=torch.bfloat16)
+        B.expert_linear(new(0, 16), w, plan, y, gather=gather)
+        B.expert_linear_backward(new(0, 16), w, plan, y, dx=new(0, 16), gather=gather, workspace=ws)
+        B.expert_linear_backward(new(0, 16), w, plan, y, dweight=dw, dbias=db, gather=gather, workspace=ws)
+        assert not dw.any() and not db.any()
+    B.linear_backward(new(0, 16), w[0], y, dx=new(0, 16), workspace=ws)
+    B.linear_backward(new(0, 16), w[0], y, dx=new(0, 16), preact=y, activation="gelu", workspace=ws)
+
+
+def test_the_same_expert_twice(B, status):
+    """A token that names one expert in two slots has two rows there; both count."""
+    t, n, width = 10, 40, 64
+    ids = torch.tensor([[1, 1, 0]] * t, dtype=torch.int32, device="cuda")
+    plan = planned(B, ids, 3)
+    x, w = rand(1, t, width), rand(2, 3, n, width, scale=0.125)
+    y, out = torch.empty(3 * t, n, device="cuda", dtype=torch.bfloat16), torch.empty(t, n, device="cuda", dtype=torch.bfloat16)
+    B.expert_linear(x, w, plan, y, gather=True, status=status)
+    weights = torch.tensor([[0.5, 0.25, 2.0]] * t, device="cuda")
+    B.expert_combine(y, plan, out, weights=weights)
+    want = 0.75 * (x.double() @ w[1].double().T) + 2.0 * (x.double() @ w[0].double().T)
+    size = 0.75 * (x.double().abs() @ w[1].double().abs().T) + 2.0 * (x.double().abs() @ w[0].double().abs().T)
+    # every row is stored once on the way: 2^-8 of each, and the sums of both steps
+    rows = 0.75 * (x.double() @ w[1].double().T).abs() + 2.0 * (x.double() @ w[0].double().T).abs()
+    bounded(out, want, 2.0 ** -8 * rows + 2 * (width + 6) * E * size + store(want, torch.bfloat16), "out")
 
 
 def test_results_past_32_bits(B, status):
