@@ -164,6 +164,7 @@ def lib():
         size = ctypes.c_size_t
         f32 = ctypes.c_float
         signatures = {
+            "ftb_debug_pair_shared_bytes": (size, [size]),
             "ftb_linear": (i32, [i32] + [vp] * 6 + [i64] * 3 + [i32, i32, cfgp, vp, vp]),
             "ftb_linear_backward_workspace_bytes": (size, [i64] * 3 + [i32]),
             "ftb_linear_backward": (i32, [i32] + [vp] * 7 + [i64] * 3 + [i32, i32, vp, size, vp, vp]),
@@ -185,7 +186,8 @@ def lib():
 
 EXPORTED_SYMBOLS = (
     "ftb_version", "ftb_strerror", "ftb_last_cuda_error", "ftb_device_check", "ftb_validate",
-    "ftb_launch_count", "ftb_selftest_bounded_wait", "ftb_debug_wait_profile", "ftb_gemm_f32", "ftb_bgemm_f32", "ftb_bgemm_bf16", "ftb_bgemm_bf16_multi", "ftb_gemm_s8",
+    "ftb_launch_count", "ftb_selftest_bounded_wait", "ftb_debug_wait_profile",
+    "ftb_debug_pair_shared_bytes", "ftb_gemm_f32", "ftb_bgemm_f32", "ftb_bgemm_bf16", "ftb_bgemm_bf16_multi", "ftb_gemm_s8",
     "ftb_conv2d_workspace_bytes", "ftb_conv2d_nchw_f32", "ftb_conv2d_nchw_f32_noalloc", "ftb_dwconv2d_nchw_f32",
     "ftb_dwconv2d_nchw_f32_multi", "ftb_conv2d_nchw_f32_multi", "ftb_conv2d_pack_filter",
     "ftb_conv2d_nchw_f32_prepacked", "ftb_conv3d_workspace_bytes", "ftb_conv3d_ncdhw_f32",

@@ -100,6 +100,8 @@ int ftb_selftest_bounded_wait(int* status, void* stream) {
   return FTB_OK;
 }
 
+size_t ftb_debug_pair_shared_bytes(size_t need) { return ftb::pair_shared_bytes(need); }
+
 int ftb_version(void) { return FTB_VERSION; }
 
 const char* ftb_strerror(int code) {

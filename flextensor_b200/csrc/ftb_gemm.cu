@@ -223,7 +223,8 @@ template <int KIND, int OUT, bool SPLIT3, bool PAIR, bool WIDE = false>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const StoreMaps& tc, const UmmaParams& p,
                   int ctas, cudaStream_t stream) {
   auto kern = umma_gemm_kernel<KIND, OUT, SPLIT3, PAIR, WIDE>;
-  const size_t smem = smem_needed(p.b_bytes / 128, p.stages, SPLIT3, p.tma_store ? kEpilogueStaging : 0);
+  size_t smem = smem_needed(p.b_bytes / 128, p.stages, SPLIT3, p.tma_store ? kEpilogueStaging : 0);
+  if (PAIR) smem = pair_shared_bytes(smem);
   // The opt-in shared-memory size is a per-device attribute of the function.
   static std::mutex mu;
   static bool done[64] = {false};
@@ -1105,7 +1106,7 @@ static int launch_slab(const CUtensorMap& tin, const CUtensorMap& tw, const Stor
   memset(&lc, 0, sizeof(lc));
   lc.gridDim = dim3(static_cast<unsigned>(sp.ctas), 1, 1);
   lc.blockDim = dim3(sp.gather ? 480 : 224, 1, 1);
-  lc.dynamicSmemBytes = sp.smem;
+  lc.dynamicSmemBytes = sp.pair ? pair_shared_bytes(sp.smem) : sp.smem;
   lc.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -16,6 +16,17 @@ int sm_count();
 // Device address of the library's own status word, used when the caller passes none.
 int* fallback_status();
 
+// Shared memory that a CTA of a pair (cta_group::2) asks for.  A pair takes tensor memory on both of its SMs before its
+// CTAs meet at a cluster barrier, and nothing says that the two are taken at once: two pairs on the same two SMs, of one
+// kernel or of any two on different streams, could each hold the columns that the other waits for.  So every pair asks
+// for more than half of an SM's shared memory, and no SM ever holds CTAs of two pairs.  (Single CTAs and split clusters may
+// stand beside a pair: they hold tensor memory without waiting for another CTA, and give it back.)
+constexpr size_t kSmSharedBytes = 228 * 1024;  // of an SM, of which the system keeps 1 KB per resident CTA
+constexpr size_t kCtaReserved = 1024;
+constexpr size_t kPairSharedFloor = 114 * 1024;
+static_assert(2 * (kPairSharedFloor + kCtaReserved) > kSmSharedBytes, "two CTAs of pairs must not fit an SM");
+inline size_t pair_shared_bytes(size_t need) { return need < kPairSharedFloor ? kPairSharedFloor : need; }
+
 // Options of gemm_generic beyond the plain (batched) product.
 struct GemmExtras {
   int a_broadcast;        // 1: every batch entry multiplies the same A (A holds one matrix)

@@ -1064,9 +1064,7 @@ int launch_linear_umma(const LinArgs& q, const ftb_config* cfg, int* status, cud
   }
 
   size_t smem = static_cast<size_t>(stages) * stage_size(c) + 1024 + turn_bytes(c);
-  // A pair holds tensor memory while its CTAs wait for each other.  No other kernel with tensor memory may share the SM
-  // with it (each could wait for columns that the other holds), so it always asks for most of the shared memory.
-  if (c.pair && smem < 176 * 1024) smem = 176 * 1024;
+  if (c.pair) smem = pair_shared_bytes(smem);
   const bool rich = q.gated || q.act || q.bias || q.residual || q.preact;
   if (c.split > 1) {
     const int ctas = static_cast<int>(most) * c.split;

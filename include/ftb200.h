@@ -110,6 +110,11 @@ int ftb_selftest_bounded_wait(int* status, void* stream);
  * of the pipeline a kernel is waiting on; no counterpart in the reference. */
 int ftb_debug_wait_profile(uint64_t* cycles, int reset);
 
+/* Dynamic shared memory that a CTA of a two-CTA tile is launched with when its stages need `need` bytes: always more than
+ * half of an SM's, so that two pairs (of one kernel, or of two kernels on two streams) never share an SM, where each could
+ * hold tensor memory that the other waits for.  For tests; no counterpart in the reference. */
+size_t ftb_debug_pair_shared_bytes(size_t need);
+
 /* GEMM entry points: operands whose row pitch or base address is not a multiple of 16 bytes cannot
  * be read by TMA; such calls are served by a CUDA-core kernel (correct, roughly 10x slower; plain
  * fp32 arithmetic for fp32 inputs).  Everything else runs on the tcgen05 kernel. */

@@ -36,6 +36,24 @@ def test_version_and_strerror(native_lib):
     assert native_lib.ftb_strerror(-99) == b"unknown error"
 
 
+def test_two_pairs_never_share_an_sm(native_lib):
+    """A pair holds tensor memory on one SM while it waits for it on another.  The smallest pair tile (32 columns, two
+    stages: 37 KB) beside any other one must not fit the 228 KB of an SM, 1 KB of which goes to each CTA."""
+    def asked(need):
+        return native_lib.ftb_debug_pair_shared_bytes(need) + 1024
+    smallest = 2 * (16384 + 16 * 128) + 1024
+    largest = 227 * 1024 - 2048
+    for need in (0, smallest, 64 << 10, 113 << 10, 114 << 10, 160 << 10, 176 << 10, largest):
+        assert asked(need) >= need + 1024 and asked(need) <= 227 * 1024
+        assert asked(need) + asked(smallest) > 228 * 1024, need
+    # every kernel that allocates for a pair is launched with that size
+    csrc = os.path.join(ROOT, "flextensor_b200", "csrc")
+    pair_kernels = [f for f in os.listdir(csrc) if f.endswith((".cu", ".cuh")) and f != "ftb_ptx.cuh" and
+                    "tmem_alloc_pair(" in open(os.path.join(csrc, f)).read()]
+    launches = sum(open(os.path.join(csrc, f)).read().count("pair_shared_bytes(") for f in ("ftb_gemm.cu", "ftb_linear_umma.cu"))
+    assert len(pair_kernels) == launches == 3, pair_kernels
+
+
 def test_config_struct_layout():
     assert ctypes.sizeof(backend.FtbConfig) == 16 * 4
     cfg = backend.FtbConfig.from_dict({"tile_n": 128, "cluster": 2, "stages": 5})
