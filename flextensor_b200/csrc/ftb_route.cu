@@ -374,10 +374,17 @@ __global__ void __launch_bounds__(256, VPL <= 4 ? 8 : VPL == 8 ? 5 : 1) route_ke
         c[v] = clean(c[v] + b[v]);
       }
     }
-    // The exponentials and reciprocals are good to a few units of 2^-24 of the largest score (their error grows with
-    // |x|, where the score's slope has vanished faster), a sum over the row to about 8 more, and the place takes
-    // VPL units of a value of up to twice that.
-    const float tol = (3e-6f + VPL * 2.4e-7f) * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(most)));
+    // What two compared values may be off by, relative to `most`.  softmax: the largest score is at least 1 / experts of
+    // the sum, its exponential and those below it are good to 2 units of 2^-23 of themselves, the sum over the row to
+    // about 8.  sigmoid: the fast exponential is good to 2 + 1.173 |x| units of 2^-23, the reciprocal to 2, so a score is
+    // off by at most 1.4e-6 of the largest one while that is at least sigmoid(-6.2) = 2e-3 (scores below it are off by
+    // more of themselves, but they are smaller by more than that); two of them by 2.8e-6, two sums of two by 5.6e-6, and
+    // adding the bias and the two rounds each value by 2^-24 of up to 4 `most`.  Where every score is smaller and no bias
+    // is larger, the bound is lost (at -87.3 the reciprocal is 0) and 64 bits decide.  The place takes VPL units of a value
+    // of up to twice `most`.
+    most = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(most)));
+    const float tol = (3.2e-6f + VPL * 2.4e-7f) * most;
+    near = sigmoid && most < 2e-3f;
     uint32_t left = avail;
     if (p.groups > 1 && p.group_lanes == 0) left = keep_groups<float, VPL>(p, c, avail, 2.0f * tol, lane, &near);
 #pragma unroll

@@ -1,0 +1,68 @@
+"""The feed-forward operators where their arithmetic is weakest: scores far below one, the tail of GELU, finite values whose
+powers overflow, rows that a plan does not fill.  Definitions, bounds and helpers as in ``test_gpu_lm``."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_lm import B, E, STEP, act64, bounded, dz64, rand, route64, scores64, slope64, status  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- scores far below one
+def routed(B, logits, k, **settings):
+    ids = torch.full((logits.shape[0], k), -7, device="cuda", dtype=torch.int32)
+    weights = torch.full((logits.shape[0], k), float("nan"), device="cuda")
+    B.route_experts(logits, ids, weights, **settings)
+    return ids, weights
+
+
+def test_route_groups_of_vanishing_scores(B):
+    """sigmoid(-87.4) + sigmoid(-87.4) = 2.2e-38 against sigmoid(-87.3) + sigmoid(-95) = 1.2e-38."""
+    logits = torch.tensor([[-87.4, -87.4, -87.3, -95.0], [-87.3, -95.0, -87.4, -87.4]], device="cuda")
+    ids, weights = routed(B, logits, 2, scoring="sigmoid", groups=2, top_groups=1)
+    assert ids.tolist() == [[0, 1], [2, 3]]
+    assert torch.allclose(weights, torch.full((2, 2), 0.5, device="cuda"), atol=1e-6)
+
+
+@pytest.mark.parametrize("e,groups", [(32, 2), (64, 2), (60, 3), (256, 4)])
+@pytest.mark.parametrize("bias", [None, "zeros", "tiny"])
+def test_route_group_sums_of_low_scores(B, e, groups, bias):
+    """Rows of logits between -95 and -6 whose groups' sums differ by less than the error of a fast exponential there (it
+    grows with the logit): each group has two logits a few fp32 steps from the other groups', and nothing else near."""
+    t, size = 8192, e // groups
+    gen = torch.Generator().manual_seed(e + groups)
+    level = -6 - 89 * torch.rand(t, 1, generator=gen, dtype=torch.float64)
+    step = 2.0 ** (torch.floor(torch.log2(-level)) - 23)
+    logits = (level - 12).expand(t, e).reshape(t, groups, size).clone()
+    first = torch.randint(-6, 7, (t, groups), generator=gen)
+    second = torch.randint(-2, 3, (t, groups), generator=gen) - first
+    logits[:, :, 1] = level + step * first
+    logits[:, :, size - 1] = level - 0.25 + step * second
+    logits = logits.reshape(t, e).float().cuda()
+    b = None
+    if bias is not None:
+        b = torch.zeros(e, device="cuda")
+        if bias == "tiny":  # one that moves nothing but the highest rows
+            b[::3] = 2.0 ** -40
+    ids, weights = routed(B, logits, 2, bias=b, scoring="sigmoid", groups=groups, top_groups=1)
+    want_ids, want = route64(logits, 2, b, "sigmoid", groups, 1, True, 1.0)
+    assert torch.equal(ids, want_ids), int((ids != want_ids).any(1).sum())
+    bounded(weights, want, (32 + e / 8) * E * want.abs(), "weights")
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (4, 2)])
+def test_route_rows_over_a_wide_range(B, scoring, dtype, groups, top_groups):
+    """Levels from -95 to 30 with spreads from a hundredth to ten: every regime of both scorings."""
+    t, e, k = 1024, 64, 6
+    gen = torch.Generator().manual_seed(11)
+    level = 30 - 125 * torch.rand(t, 1, generator=gen)
+    spread = 10.0 ** (1 - 3 * torch.rand(t, 1, generator=gen))
+    logits = (level + spread * torch.randn(t, e, generator=gen)).to(dtype).cuda()
+    ids, weights = routed(B, logits, k, scoring=scoring, groups=groups, top_groups=top_groups)
+    want_ids, want = route64(logits, k, None, scoring, groups, top_groups, True, 1.0)
+    assert torch.equal(ids, want_ids), int((ids != want_ids).any(1).sum())
+    bounded(weights, want, (32 + e / 8) * E * want.abs() + 1e-37, "weights")
