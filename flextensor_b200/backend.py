@@ -846,8 +846,9 @@ def expert_linear(x, weight, plan, out, bias=None, activation="none", gated=Fals
     """For every place p of expert e in ``plan``: out[p] = act(x-row @ weight[e].T + bias[e]), gated as in ``linear``.
 
     weight [E,N,K] (gated [E,2N,K]), bias [E,N] ([E,2N]), out [rows,N], preact [rows,N] ([rows,2N]).  ``gather``: x is
-    [tokens,K] and place p reads its token's row; otherwise x is [rows,K], sorted.  Places past the last row
-    (``plan.offsets[-1]``) are left as they were.
+    [tokens,K] and place p reads its token's row (a row of zeros where ``plan.order`` names none, which plans of
+    ``expert_plan`` never do); otherwise x is [rows,K], sorted.  Places past the last row (``plan.offsets[-1]``) are left as
+    they were.
     """
     dtype = _element(x, "x")
     act = _one_of(activation, ACTIVATIONS, "activation")

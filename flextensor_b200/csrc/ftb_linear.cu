@@ -155,14 +155,15 @@ expert_rows_kernel(const uint16_t* __restrict__ x, const int* __restrict__ offse
   grid_launch_dependents();
   const long long place = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (place >= rows || place >= offsets[groups]) return;
+  // a place of an expert's run that names no row is a row of zeros, as in the forward product (gathered_row)
   const int o = order[place];
   const long long row = o < 0 ? src_rows : o / div;
-  if (row >= src_rows) return;
+  const bool there = row < src_rows;
   const uint16_t* src = x + row * k;
   uint16_t* dst = sorted + place * k;
   for (long long c = static_cast<long long>(threadIdx.x & 31) * VEC; c < k; c += 32 * VEC) {
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-    else dst[c] = src[c];
+    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(dst + c) = there ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0, 0, 0, 0);
+    else dst[c] = there ? src[c] : static_cast<uint16_t>(0);
   }
 }
 

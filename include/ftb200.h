@@ -314,7 +314,8 @@ int ftb_expert_plan(const int32_t* ids, int32_t* offsets, int32_t* order, int32_
                     void* stream);
 
 /* For every sorted place p of expert e: out[p,n] = epilogue of ftb_linear (no residual) over x-row . w[e]^T + bias[e].
- * gather = 1: x is [rows / top_k, k] and place p reads row order[p] / top_k; gather = 0: x is [rows, k], sorted.
+ * gather = 1: x is [rows / top_k, k] and place p reads row order[p] / top_k (a row of zeros, here and in the gradients,
+ * where order[p] names none); gather = 0: x is [rows, k], sorted.
  * w[experts, n or 2n, k], bias[experts, n or 2n].  Places past offsets[experts] are left as they were in out and preact.
  * Knobs as for ftb_linear, without split_k. */
 int ftb_expert_linear(int dtype, const void* x, const void* w, const void* bias, const int32_t* offsets,

@@ -66,3 +66,36 @@ def test_route_rows_over_a_wide_range(B, scoring, dtype, groups, top_groups):
     want_ids, want = route64(logits, k, None, scoring, groups, top_groups, True, 1.0)
     assert torch.equal(ids, want_ids), int((ids != want_ids).any(1).sum())
     bounded(weights, want, (32 + e / 8) * E * want.abs() + 1e-37, "weights")
+
+
+# ---------------------------------------------------------------- plans that the caller made
+@pytest.mark.parametrize("width", [72, 20])
+def test_places_without_a_row(B, status, width):
+    """A place inside an expert's run whose order names no row (-1, or one past the tokens) is a row of zeros, forward and
+    backward, whatever the workspace held."""
+    t, k, e, n = 12, 2, 3, 40
+    order = torch.arange(t * k, dtype=torch.int32)
+    order[3], order[4], order[13] = -1, t * k, 2 ** 31 - 1
+    offsets = torch.tensor([0, 9, 9, 20], dtype=torch.int32)
+    slots = torch.full((t * k,), -1, dtype=torch.int32)
+    plan = B.ExpertPlan.over(t, k, e, offsets.cuda(), order.cuda(), slots.cuda())
+    x, w, b = rand(1, t, width), rand(2, e, n, width, scale=0.2), rand(3, e, n)
+    dy = rand(4, t * k, n)
+    rows = torch.zeros(20, width, device="cuda", dtype=torch.float64)
+    for place in range(20):
+        if 0 <= int(order[place]) < t * k:
+            rows[place] = x[int(order[place]) // k].double()
+    out = torch.full((t * k, n), 7.0, device="cuda", dtype=torch.bfloat16)
+    B.expert_linear(x, w, plan, out, bias=b, gather=True, status=status)
+    dx, dw, db = torch.full((t * k, width), 7.0, device="cuda", dtype=torch.bfloat16), torch.empty_like(w), torch.empty_like(b)
+    ws = torch.full((B.expert_linear_backward_workspace_bytes(plan, n, width),), 255, dtype=torch.uint8, device="cuda")  # NaN
+    B.expert_linear_backward(x, w, plan, dy, dx=dx, dweight=dw, dbias=db, gather=True, workspace=ws, status=status)
+    for i, (a, c) in enumerate(((0, 9), (9, 9), (9, 20))):
+        z = rows[a:c] @ w[i].double().T + b[i].double()
+        size = rows[a:c].abs() @ w[i].double().abs().T + b[i].double().abs()
+        bounded(out[a:c], z, 2 * (width + 2) * E * size + STEP[torch.bfloat16] * z.abs(), "out %d" % i)
+        g = dy[a:c].double()
+        want = g.T @ rows[a:c]
+        bounded(dw[i], want, 2 * 32 * E * (g.abs().T @ rows[a:c].abs()) + STEP[torch.bfloat16] * want.abs(), "dw %d" % i)
+        bounded(db[i], g.sum(0), 100 * E * g.abs().sum(0) + STEP[torch.bfloat16] * g.sum(0).abs(), "db %d" % i)
+    assert (out[20:] == 7).all() and (dx[20:] == 7).all()
