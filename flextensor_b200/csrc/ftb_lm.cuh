@@ -49,14 +49,21 @@ constexpr float kGeluA = 0.044715f;
 // 1 / (1 + exp(-x)); exp overflows to infinity for very negative x, which gives the limit 0.
 __device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
-// Phi(z), the normal distribution function, and exp(-z^2/2) on the way: Abramowitz and Stegun 7.1.26 (erf to 1.5e-7),
-// one reciprocal and one exponential; the tail of a negative z is the product itself, without cancellation.
+// Phi(z), the normal distribution function, and exp(-z^2/2) on the way.  Phi(-|z|) exp(z^2/2) is smooth in
+// t = 1 / (1 + 0.36 |z|) and goes to 0 with it: t times a polynomial of degree 6, whose coefficients minimise the largest
+// RELATIVE error for |z| up to 14.5 (a linear program over 1200 nodes; 9.5e-7), so the tail of a negative z is the product
+// itself and keeps fp32's digits: in fp32 off by 1.4e-6 of itself to z = -3, 3.7e-6 to -8, 6.8e-6 to -13, where the exponent's
+// rounding leads, far below half a step of a 16-bit result (2^-11).
 __device__ __forceinline__ float normal_cdf(float z, float* bell) {
-  const float x = fabsf(z) * 0.7071067811865476f;
-  const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-  const float e = __expf(-x * x);
-  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float tail = 0.5f * poly * e;
+  const float t = __fdividef(1.0f, fmaf(0.36f, fabsf(z), 1.0f));
+  const float e = __expf(-0.5f * z * z);
+  float poly = fmaf(t, 0.046779383f, -0.178817928f);
+  poly = fmaf(t, poly, 0.179667756f);
+  poly = fmaf(t, poly, 0.0274331067f);
+  poly = fmaf(t, poly, 0.139397204f);
+  poly = fmaf(t, poly, 0.141831115f);
+  poly = fmaf(t, poly, 0.1437089f);
+  const float tail = t * poly * e;
   *bell = e;
   return z < 0.0f ? tail : 1.0f - tail;
 }

@@ -99,3 +99,48 @@ def test_places_without_a_row(B, status, width):
         bounded(dw[i], want, 2 * 32 * E * (g.abs().T @ rows[a:c].abs()) + STEP[torch.bfloat16] * want.abs(), "dw %d" % i)
         bounded(db[i], g.sum(0), 100 * E * g.abs().sum(0) + STEP[torch.bfloat16] * g.sum(0).abs(), "db %d" % i)
     assert (out[20:] == 7).all() and (dx[20:] == 7).all()
+
+
+# ---------------------------------------------------------------- GELU's tail
+def tail(dtype):
+    """z from -3 to -8 (fp16: to -5, where its results end), exact in the type."""
+    z = -torch.linspace(3, 8 if dtype == torch.bfloat16 else 5, 512)
+    return z.to(dtype).cuda()
+
+
+def relative(got, want, dtype, what):
+    """Half a step of the result's type, and 2^-16 of the value for the arithmetic: the exponent of the bell is z^2 / 2 with
+    two roundings of 2^-24, 2^-18.2 of the value at z = -8, the fast exponential adds 2^-22 + |z^2 / 2| 2^-24 (2^-18.9) and
+    the rest a few 2^-22.  fp16 has a smallest step of 2^-24."""
+    bounded(got, want, (STEP[dtype] + 2.0 ** -16) * want.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0), what)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_gelu_tail(B, status, dtype, gated):
+    z = tail(dtype)
+    n = z.numel()
+    w = torch.zeros(n * (2 if gated else 1), 64, device="cuda", dtype=dtype)
+    w[:n, 0] = z
+    if gated:
+        w[n:, 0] = 4.0
+    x = torch.zeros(3, 64, device="cuda", dtype=dtype)
+    x[:, 0] = 1
+    for cfg in (None, {"tile_n": 16, "split_k": 1}, {"cluster": 2}):
+        out = torch.empty(3, n, device="cuda", dtype=dtype)
+        B.linear(x, w, out, activation="gelu", gated=gated, cfg=cfg, status=status)
+        want = act64(z.double(), "gelu") * (4 if gated else 1)
+        relative(out, want.expand(3, n), dtype, "gelu")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_slope_in_the_tail(B, status, dtype):
+    """The bias gradient of one token is act'(z) itself, rounded once."""
+    z = tail(dtype)[None]
+    n = z.shape[1]
+    dy = torch.ones(1, n, device="cuda", dtype=dtype)
+    db = torch.empty(n, device="cuda", dtype=dtype)
+    ws = torch.empty(B.linear_backward_workspace_bytes(1, n, 64), dtype=torch.uint8, device="cuda")
+    B.linear_backward(rand(1, 1, 64, dtype=dtype), rand(2, n, 64, dtype=dtype), dy, dbias=db, preact=z, activation="gelu",
+                      workspace=ws, status=status)
+    relative(db, slope64(z[0].double(), "gelu"), dtype, "slope")
