@@ -104,11 +104,12 @@ __device__ __forceinline__ void act_both(const float (&z)[N], float (&value)[N],
       slope[i] = fmaf(z[i] * 0.3989422804014327f, bell, cdf);
     }
   } else if (act == FTB_ACT_GELU_TANH) {
+    // z^2 is held to 1e4 (s is 0 or 1 from |z| = 15 on), so that no power of a large finite z becomes 0 * inf
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float q = z[i] * z[i], s = sigmoid_f(2.0f * kGeluC * z[i] * fmaf(kGeluA, q, 1.0f));
+      const float q = fminf(z[i] * z[i], 1e4f), s = sigmoid_f(2.0f * kGeluC * z[i] * fmaf(kGeluA, q, 1.0f));
       value[i] = z[i] * s;
-      slope[i] = fmaf(2.0f * z[i] * s * (1.0f - s) * kGeluC, fmaf(3.0f * kGeluA, q, 1.0f), s);
+      slope[i] = fmaf(z[i] * (s * (1.0f - s)), 2.0f * kGeluC * fmaf(3.0f * kGeluA, q, 1.0f), s);
     }
   } else if (act == FTB_ACT_RELU) {
 #pragma unroll

@@ -144,3 +144,27 @@ def test_gelu_slope_in_the_tail(B, status, dtype):
     B.linear_backward(rand(1, 1, 64, dtype=dtype), rand(2, n, 64, dtype=dtype), dy, dbias=db, preact=z, activation="gelu",
                       workspace=ws, status=status)
     relative(db, slope64(z[0].double(), "gelu"), dtype, "slope")
+
+
+# ---------------------------------------------------------------- finite values whose powers overflow
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_huge_preactivations(B, status, act, gated):
+    """z up to the type's largest: every activation is z or 0 there and its slope 1 or 0, without a NaN on the way."""
+    huge = torch.tensor([1e4, 1e10, 2e13, 1e19, 2e19, 1e25, 1e30, 3e38] * 8).to(torch.bfloat16)
+    z = torch.cat([huge, -huge])[None].cuda()
+    n = z.shape[1]
+    zz = torch.cat([z, torch.full_like(z, 0.5)], dim=1) if gated else z
+    w = torch.zeros(zz.shape[1], 64, device="cuda", dtype=torch.bfloat16)
+    w[:, 0] = zz[0]
+    x = torch.zeros(1, 64, device="cuda", dtype=torch.bfloat16)
+    x[:, 0] = 1
+    out = torch.empty(1, n, device="cuda", dtype=torch.bfloat16)
+    B.linear(x, w, out, activation=act, gated=gated, status=status)
+    want = act64(z.double(), act) * (0.5 if gated else 1)
+    bounded(out, want, STEP[torch.bfloat16] * want.abs(), act)
+    dy, db = torch.ones_like(out), torch.empty(zz.shape[1], device="cuda", dtype=torch.bfloat16)
+    ws = torch.empty(B.linear_backward_workspace_bytes(1, n, 64, gated), dtype=torch.uint8, device="cuda")
+    B.linear_backward(x, w, dy, dbias=db, preact=zz, activation=act, gated=gated, workspace=ws, status=status)
+    want = dz64(dy, zz, act, gated)[0]
+    bounded(db, want, STEP[torch.bfloat16] * want.abs(), act + " slope")
