@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256, VPL <= 4 ? 8 : VPL == 8 ? 5 : 1) route_ke
 // d logits.  With the chosen scores scaled to one, r = s / S with S the sum of the chosen s, softmax gives
 //   dl_j = r_j g_j with g_j = scale (dw_j - sum_i r_i dw_i)
 // for the chosen (the row's other logits cancel), and sigmoid dl_j = r_j g_j (1 - s_j), taken as (dw_j - sum dw s / S) / S s_j
-// while S does not underflow and by the ratios of exp(l) below that.  Without scaling softmax gives dl_e = s_e (g_e -
+// while S is 1e-9 or more and by the ratios of exp(l) below that.  Without scaling softmax gives dl_e = s_e (g_e -
 // sum_j g_j s_j) for every expert and sigmoid dl_j = g_j s_j (1 - s_j), g = scale dw.  An expert that a row names twice gets
 // both parts, added in the order of the slots.  8192 x 128 bf16, softmax over all: 5 us of device time for 4.7 MB.
 template <typename T, int VPL>
@@ -484,10 +484,11 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs p) 
     const float s = sigmoid ? (active ? 1.0f / (1.0f + expf(-l)) : 0.0f) : 0.0f;
     if (p.renorm) {
       const float sum = sigmoid ? warp_sum(s) : 0.0f;
-      if (sum >= 1e-30f) {
+      if (sum >= 1e-9f) {
         part = (dw - warp_sum(dw * s) / sum) / sum * s;
       } else {
-        // softmax, or scores that underflow: by the ratios of exp(l)
+        // softmax, or scores below 1e-9, which are exp(l) to 1e-9 of themselves: by the ratios of exp(l), so that neither
+        // dw s leaves the range of fp32 nor dw / sum
         const float top = warp_max(l);
         float r = active ? exp_below(l, top) : 0.0f;
         const float total_r = warp_sum(r);

@@ -168,3 +168,21 @@ def test_huge_preactivations(B, status, act, gated):
     B.linear_backward(x, w, dy, dbias=db, preact=zz, activation=act, gated=gated, workspace=ws, status=status)
     want = dz64(dy, zz, act, gated)[0]
     bounded(db, want, STEP[torch.bfloat16] * want.abs(), act + " slope")
+
+
+@pytest.mark.parametrize("level", [-12.0, -25.0, -45.0, -62.0, -68.0, -75.0])
+@pytest.mark.parametrize("size", [1e-20, 1e-13, 1.0, 1e12])
+def test_route_backward_of_low_scores(B, level, size):
+    """Scaled sigmoid weights: their gradient is that of a softmax over the chosen logits however small the scores and the
+    incoming gradients are; no product of the two may leave the range of fp32 on the way."""
+    t, e, k = 40, 64, 6
+    logits = rand(5, t, e, dtype=torch.float32) * 0.5 + level
+    ids, _ = routed(B, logits, k, scoring="sigmoid")
+    dweights = rand(6, t, k, dtype=torch.float32) * size
+    got = torch.full_like(logits, float("nan"))
+    B.route_experts_backward(logits, ids, dweights, got, scoring="sigmoid")
+    x = logits.double().requires_grad_(True)
+    w = torch.sigmoid(x).gather(1, ids.long())
+    want = torch.autograd.grad((w / w.sum(1, keepdim=True) * dweights).sum(), x)[0]
+    # as in test_route_backward: a few steps of the row's largest term, which may cancel
+    bounded(got, want, (64 + e / 4) * E * dweights.double().abs().amax(1, keepdim=True), "dlogits")
