@@ -602,7 +602,7 @@ def dwconv2d_nchw_f32_multi(x, weight, dst_ptrs, bias=None, stride=(1, 1), paddi
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 SCORINGS = {"softmax": 0, "sigmoid": 1}
-MAX_EXPERTS, MAX_TOP_K = 1024, 32
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 32, 32
 _ELEMENTS = (torch.bfloat16, torch.float16)
 
 

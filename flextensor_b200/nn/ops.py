@@ -23,6 +23,7 @@ reference's ``flextensor/nn/ops.py``:
 The reference is fp32 only; ``dtype`` follows the input tensors here so that the same
 index expressions serve bf16 (fp32 accumulate) and int8 (int32 accumulate).
 """
+from ..backend import MAX_EXPERTS, MAX_GROUPS, MAX_TOP_K
 from ..ir import ComputeOp, Tensor, reduce_axis
 from ..utils import assert_print
 
@@ -337,7 +338,13 @@ def linear(x, weight, bias=None, residual=None, activation="none", gated=False):
 
 def route_experts(logits, top_k, bias=None, scoring="softmax", groups=1, top_groups=1, renormalize=True, scale=1.0):
     """(ids, weights), both [T, top_k]: the experts of every token and their weights (``backend.route_experts``)."""
+    assert_print(logits.ndim == 2 and logits.dtype in ("float32", "bfloat16", "float16"),
+                 "logits are [T, E] in float32, bfloat16 or float16")
     t, e = (int(s) for s in logits.shape)
+    assert_print(1 <= e <= MAX_EXPERTS and top_k <= MAX_TOP_K and groups <= MAX_GROUPS,
+                 "at most %d experts, top_k %d and %d groups" % (MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS))
+    if bias is not None:
+        assert_print([int(s) for s in bias.shape] == [e] and bias.dtype == "float32", "bias is [E] in float32")
     assert_print(1 <= top_groups <= groups and e % groups == 0 and 1 <= top_k <= e // groups * top_groups,
                  "top_k %d of %d experts in %d groups, %d kept" % (top_k, e, groups, top_groups))
     assert_print(scoring in ("softmax", "sigmoid"), "scoring must be softmax or sigmoid")
@@ -351,8 +358,10 @@ def route_experts(logits, top_k, bias=None, scoring="softmax", groups=1, top_gro
 
 def expert_plan(ids, experts):
     """(offsets [experts+1], order [T*top_k], slots [T*top_k]): rows of ids [T, top_k] sorted by expert."""
+    assert_print(ids.ndim == 2 and ids.dtype == "int32", "ids are [T, top_k] in int32")
     t, top_k = (int(s) for s in ids.shape)
-    assert_print(ids.dtype == "int32", "ids are int32")
+    assert_print(1 <= experts <= MAX_EXPERTS and 1 <= top_k <= MAX_TOP_K,
+                 "1 to %d experts and top_k of 1 to %d" % (MAX_EXPERTS, MAX_TOP_K))
     op = ComputeOp("expert_plan", "expert_plan", (experts + 1,), "int32", [ids], ("e",),
                    attrs={"tokens": t, "top_k": top_k, "experts": int(experts)},
                    more_outputs=[((t * top_k,), "int32"), ((t * top_k,), "int32")])
@@ -360,7 +369,8 @@ def expert_plan(ids, experts):
 
 
 def _plan_attrs(plan):
-    assert_print(len(plan) == 3 and getattr(plan[0].op, "kind", None) == "expert_plan", "plan is what expert_plan returned")
+    assert_print(len(plan) == 3 and getattr(plan[0].op, "kind", None) == "expert_plan" and
+                 all(t is plan[0].op.output(i) for i, t in enumerate(plan)), "plan is what expert_plan returned")
     return dict(plan[0].op.attrs)
 
 
@@ -381,9 +391,14 @@ def expert_linear(x, weight, plan, bias=None, activation="none", gated=False, ga
 def expert_combine(y, plan, weights=None, residual=None):
     """out[t,i] = residual[t,i] + sum_j weights[t,j] * y[place of (t, j), i]; dropped rows add nothing."""
     sizes = _plan_attrs(plan)
+    assert_print(y.ndim == 2 and y.dtype in ("bfloat16", "float16"), "y is [T * top_k, N] in bfloat16 or float16")
     rows, n = (int(s) for s in y.shape)
     t, top_k = sizes["tokens"], sizes["top_k"]
     assert_print(rows == t * top_k, "y has %d rows" % rows)
+    if weights is not None:
+        assert_print([int(s) for s in weights.shape] == [t, top_k] and weights.dtype == "float32", "weights are [T, top_k] in float32")
+    if residual is not None:
+        assert_print([int(s) for s in residual.shape] == [t, n] and residual.dtype == y.dtype, "residual of shape %s" % (residual.shape,))
     names, tensors = _operands(y=y, weights=weights, residual=residual)
     op = ComputeOp("expert_combine", "expert_combine", (t, n), y.dtype, tensors + list(plan), ("t", "i"),
                    reduce_axes=[reduce_axis((0, top_k), name="j")],

@@ -54,6 +54,29 @@ def test_expert_definitions():
             bad()
 
 
+def test_definitions_refuse_what_the_launchers_do():
+    """Types, shapes and limits are named when the graph is made, not at its first run."""
+    f32 = lambda *shape: placeholder(shape)
+    i32 = lambda *shape: placeholder(shape, dtype="int32")
+    plan = ops.expert_plan(i32(10, 2), 8)
+    y, other = bf(20, 64), ops.expert_plan(i32(10, 2), 8)
+    for bad in (lambda: ops.route_experts(placeholder((10, 8), dtype="int8"), 2), lambda: ops.route_experts(f32(2, 10, 8), 2),
+                lambda: ops.route_experts(f32(10, 1025), 2), lambda: ops.route_experts(f32(10, 64), 33),
+                lambda: ops.route_experts(f32(10, 66), 2, groups=33, top_groups=2),
+                lambda: ops.route_experts(f32(10, 8), 2, bias=f32(7)), lambda: ops.route_experts(f32(10, 8), 2, bias=bf(8)),
+                lambda: ops.expert_plan(i32(10, 2), 1025), lambda: ops.expert_plan(i32(10, 2), 0),
+                lambda: ops.expert_plan(i32(10, 33), 64), lambda: ops.expert_plan(f32(10, 2), 8), lambda: ops.expert_plan(i32(20), 8),
+                lambda: ops.expert_combine(f32(20, 64), plan), lambda: ops.expert_combine(y, plan, weights=f32(10, 3)),
+                lambda: ops.expert_combine(y, plan, weights=bf(10, 2)), lambda: ops.expert_combine(y, plan, residual=f32(10, 64)),
+                lambda: ops.expert_combine(y, plan, residual=bf(9, 64)),
+                lambda: ops.expert_combine(y, (plan[0], plan[2], plan[1])), lambda: ops.expert_combine(y, (plan[0], plan[1], other[2]))):
+        with pytest.raises(AssertionError):
+            bad()
+    for dtype in ("float32", "bfloat16", "float16"):
+        ops.route_experts(placeholder((10, 1024), dtype=dtype), 32, bias=f32(1024), groups=32, top_groups=32)
+    assert ops.expert_combine(y, plan, weights=f32(10, 2), residual=bf(10, 64)).dtype == "bfloat16"
+
+
 def test_graph_order_and_plan():
     """Every op comes after its producers, though the router is reached over paths of three lengths."""
     key = "experts_expert_ffn_(8, 64, 8, 2048, 1024)_cuda(0)"
