@@ -186,3 +186,94 @@ def test_route_backward_of_low_scores(B, level, size):
     want = torch.autograd.grad((w / w.sum(1, keepdim=True) * dweights).sum(), x)[0]
     # as in test_route_backward: a few steps of the row's largest term, which may cancel
     bounded(got, want, (64 + e / 4) * E * dweights.double().abs().amax(1, keepdim=True), "dlogits")
+
+
+# ---------------------------------------------------------------- rows that a mask leaves little of
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (4, 2)])
+def test_masked_rows_against_the_definition(B, scoring, dtype, groups, top_groups):
+    t, e, k = 9, 40, 4
+    logits = rand(1, t, e, dtype=dtype)
+    low = torch.finfo(dtype).min
+    logits[0, 3:] = -math.inf        # fewer experts left than wanted
+    logits[1] = -math.inf            # none left
+    logits[2, ::2] = float("nan")
+    logits[3] = low                  # the type's lowest value everywhere
+    logits[4, 5:] = low
+    logits[5, 7] = math.inf
+    logits[6] = float("nan")
+    logits[7] = -200.0               # every sigmoid underflows
+    logits[8, 10:] = -math.inf       # whole groups masked
+    clean = torch.where(logits.isnan(), -math.inf, logits.double())
+    for renorm in (True, False):
+        ids, weights = routed(B, logits, k, scoring=scoring, groups=groups, top_groups=top_groups, renormalize=renorm)
+        want_ids, want = route64(logits, k, None, scoring, groups, top_groups, renorm, 1.0)
+        if scoring == "sigmoid" and renorm:
+            # the ratios of the chosen scores where 64 bits lose the scores themselves: a softmax of log(sigmoid)
+            part = torch.nn.functional.logsigmoid(clean.gather(1, ids.long()))
+            want = torch.where(part.amax(1, keepdim=True) == -math.inf, 0.0, torch.softmax(part, 1).nan_to_num(0.0))
+        if scoring == "softmax":
+            # an infinite logit takes all of the mass (64 bits: inf - inf)
+            want_ids[5, 0] = 7
+            p5 = torch.zeros(e, dtype=torch.float64, device="cuda")
+            p5[7] = 1
+            want[5] = p5[ids[5].long()]
+        assert torch.equal(ids[[r for r in range(t) if r != 5]], want_ids[[r for r in range(t) if r != 5]])
+        assert ids[5, 0] == 7
+        assert set(ids[4].tolist()) <= set(range(10 if groups > 1 else 5))
+        bounded(weights, want, (32 + e / 8) * E * want.abs() + 1e-37, "weights")
+        # gradients: rows with a finite largest logit, by the same definition in 64 bits
+        dweights = rand(3, t, k, dtype=torch.float32)
+        back = torch.full_like(logits, float("nan"))
+        B.route_experts_backward(logits, ids, dweights, back, scoring=scoring, renormalize=renorm)
+        assert torch.isfinite(back.float()).all()
+        assert not back[1].any() and not back[6].any()
+        rows = [0, 2, 3, 4, 7, 8]
+        s = scores64(clean[rows], scoring)
+        chosen, g = s.gather(1, ids[rows].long()), dweights[rows].double()
+        r = want[rows]
+        want = torch.zeros(len(rows), e, dtype=torch.float64, device="cuda")
+        if renorm:
+            d = r * (g - (r * g).sum(1, keepdim=True))
+            want.scatter_add_(1, ids[rows].long(), d * (1 - chosen) if scoring == "sigmoid" else d)
+        elif scoring == "sigmoid":
+            want.scatter_add_(1, ids[rows].long(), g * chosen * (1 - chosen))
+        else:
+            dp = torch.zeros_like(want).scatter_add_(1, ids[rows].long(), g)
+            want = s * (dp - (dp * s).sum(1, keepdim=True))
+        bounded(back[rows], want, (64 + e / 4) * E * g.abs().amax(1, keepdim=True) + (STEP[dtype] * want.abs() + 2.0 ** -25), "dlogits")
+
+
+def test_expert_ffn_task_without_its_residual(B):
+    """The routed part of the block alone, against its own size: a lost or misplaced expert shows."""
+    from flextensor_b200.runtime import build, torch_dtype
+    from flextensor_b200.scheduler import schedule_with_config
+    from flextensor_b200.utils import Config
+    t, e, k, d, h = 8, 64, 8, 2048, 1024
+    s, bufs = schedule_with_config("experts_expert_ffn_(8, 64, 8, 2048, 1024)_cuda(0)", Config([], None))
+    func = build(s, bufs, "cuda")
+    arrays = [torch.zeros(tuple(int(v) for v in b.shape), device="cuda", dtype=torch_dtype(b.dtype)) for b in bufs]
+    x, logits, w1, w2 = arrays[:4]
+    w1.copy_(rand(3, e, 2 * h, d, scale=d ** -0.5))
+    w2.copy_(rand(4, e, d, h, scale=h ** -0.5))
+    x.copy_(rand(10, t, d))
+    logits.copy_(rand(11, t, e, dtype=torch.float32))
+    func(*arrays)
+    func.check()
+    ids, weights = route64(logits, k, None, "softmax", 1, 1, True, 1.0)
+    assert torch.equal(arrays[4], ids)
+    routed_part, size = torch.zeros(t, d, device="cuda", dtype=torch.float64), torch.zeros(t, d, device="cuda", dtype=torch.float64)
+    for i in range(e):
+        share = (weights * (ids == i)).sum(1, keepdim=True)
+        if bool((share > 0).any()):
+            z = x.double() @ w1[i].double().T
+            hidden = act64(z[:, :h], "silu") * z[:, h:]
+            y = hidden @ w2[i].double().T
+            # the hidden row and y are stored in bf16 on the way: 2^-8 of each; the first error passes w2, whose terms
+            # have independent signs: eight standard deviations
+            off = 8 * 2.0 ** -8 * (hidden.square() @ w2[i].double().square().T).sqrt()
+            routed_part += share * y
+            size += share * (2.0 ** -8 * y.abs() + off + 2.0 ** -18 * (hidden.abs() @ w2[i].double().abs().T))
+    got = arrays[-1].double() - x.double()
+    bounded(got, routed_part, size + 2.0 ** -8 * (routed_part + x.double()).abs(), "routed part")
