@@ -277,3 +277,93 @@ def test_expert_ffn_task_without_its_residual(B):
             size += share * (2.0 ** -8 * y.abs() + off + 2.0 ** -18 * (hidden.abs() @ w2[i].double().abs().T))
     got = arrays[-1].double() - x.double()
     bounded(got, routed_part, size + 2.0 ** -8 * (routed_part + x.double()).abs(), "routed part")
+
+
+# ---------------------------------------------------------------- tensors of more than 2^31 elements
+def test_expert_weights_past_32_bits(B, status):
+    """2.2e9 weights and as many of their gradient: the last expert's lie behind 2^31 of them."""
+    t, k, e, n, width = 40, 2, 33, 8200, 8192
+    ids = torch.stack([torch.arange(t) % e, torch.full((t,), e - 1)], dim=1).to(torch.int32)
+    ids[:, 0] = torch.where(ids[:, 0] == e - 1, 0, ids[:, 0])
+    plan = B.ExpertPlan(t, k, e)
+    B.expert_plan(ids.cuda(), plan)
+    x = rand(1, t, width)
+    w = torch.empty(e, n, width, device="cuda", dtype=torch.bfloat16)
+    for i in range(e):
+        w[i].normal_(0, width ** -0.5, generator=torch.Generator(device="cuda").manual_seed(i))
+    out, dy = torch.empty(t * k, n, device="cuda", dtype=torch.bfloat16), rand(2, t * k, n)
+    B.expert_linear(x, w, plan, out, gather=True, status=status)
+    dx, dw = torch.empty(t * k, width, device="cuda", dtype=torch.bfloat16), torch.empty_like(w)
+    ws = torch.empty(B.expert_linear_backward_workspace_bytes(plan, n, width), dtype=torch.uint8, device="cuda")
+    B.expert_linear_backward(x, w, plan, dy, dx=dx, dweight=dw, gather=True, workspace=ws, status=status)
+    half = STEP[torch.bfloat16]
+    for i in (0, e - 2, e - 1):
+        a, c = plan.offsets[i:i + 2].tolist()
+        rows, g, wi = x[plan.order[a:c].long() // k].double(), dy[a:c].double(), w[i].double()
+        z = rows @ wi.T
+        bounded(out[a:c], z, 2 * (width + 2) * E * (rows.abs() @ wi.abs().T) + half * z.abs(), "out")
+        want = g @ wi
+        bounded(dx[a:c], want, 2 * (n + 2) * E * (g.abs() @ wi.abs()) + half * want.abs(), "dx")
+        want = g.T @ rows
+        bounded(dw[i], want, 2 * (c - a + 2) * E * (g.abs().T @ rows.abs()) + half * want.abs(), "dw")
+
+
+def test_sorted_rows_past_32_bits(B, status):
+    """2.2e9 elements of y in the weighted sum and its gradient, and of x by place in a weight gradient."""
+    t, k, n = 41000, 2, 27000
+    plan = B.ExpertPlan(t, k, 2)
+    ids = torch.tensor([[0, 1]], dtype=torch.int32).repeat(t, 1).cuda()
+    B.expert_plan(ids, plan)
+    y = torch.empty(t * k, n, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    weights, out = torch.rand(t, k, device="cuda"), torch.empty(t, n, device="cuda", dtype=torch.bfloat16)
+    B.expert_combine(y, plan, out, weights=weights)
+    dy, dweights = torch.empty_like(y), torch.empty_like(weights)
+    B.expert_combine_backward(out, plan, y=y, weights=weights, dy=dy, dweights=dweights)
+    half = STEP[torch.bfloat16]
+    for i in (0, 20000, 39600, t - 1):
+        part = torch.stack([y[i], y[t + i]]).double()
+        terms = part * weights[i].double()[:, None]
+        bounded(out[i], terms.sum(0), 6 * E * terms.abs().sum(0) + half * terms.sum(0).abs(), "out")
+        want = out[i].double() * weights[i].double()[:, None]
+        bounded(torch.stack([dy[i], dy[t + i]]), want, E * want.abs() + half * want.abs(), "dy")
+        dots = part * out[i].double()
+        bounded(dweights[i], dots.sum(1), 2 * (n + 2) * E * dots.abs().sum(1), "dweights")
+    del y, dy, out
+    t, k, n, width = 33800, 8, 8, 8192
+    plan = B.ExpertPlan(t, k, 2)
+    ids = torch.arange(8, dtype=torch.int32).remainder(2).repeat(t, 1).cuda()
+    B.expert_plan(ids, plan)
+    x, w, dy = rand(3, t, width), rand(4, 2, n, width), rand(5, t * k, n)
+    dw = torch.empty_like(w)
+    ws = torch.empty(B.expert_linear_backward_workspace_bytes(plan, n, width), dtype=torch.uint8, device="cuda")
+    B.expert_linear_backward(x, w, plan, dy, dweight=dw, gather=True, workspace=ws, status=status)
+    for i in range(2):
+        a, c = plan.offsets[i:i + 2].tolist()
+        token = plan.order[a:c].long() // k
+        g = torch.zeros(t, n, dtype=torch.float64, device="cuda").index_add_(0, token, dy[a:c].double())
+        size = torch.zeros(t, n, dtype=torch.float64, device="cuda").index_add_(0, token, dy[a:c].double().abs())
+        want = g.T @ x.double()
+        # sums of 135200 terms: the bound of a sum one after the other is far above what is lost; their size, not it, shows
+        # a wrong row
+        bounded(dw[i], want, 2.0 ** -14 * (size.T @ x.double().abs()) + half * want.abs(), "dw")
+
+
+def test_logits_past_32_bits(B):
+    """2.15e9 logits: the last tokens' lie behind 2^31 of them."""
+    t, e, k = 2100000, 1024, 4
+    logits = torch.empty(t, e, device="cuda", dtype=torch.bfloat16)
+    logits[:-64] = -1.0
+    logits[-64:] = rand(1, 64, e)
+    logits[:64] = rand(2, 64, e)
+    ids, weights = routed(B, logits, k)
+    dweights, back = torch.ones_like(weights), torch.full_like(logits, float("nan"))
+    dweights[:, 0] = 2.0
+    B.route_experts_backward(logits, ids, dweights, back)
+    for rows in (slice(0, 64), slice(t - 64, t)):
+        want_ids, want = route64(logits[rows], k, None, "softmax", 1, 1, True, 1.0)
+        assert torch.equal(ids[rows], want_ids)
+        bounded(weights[rows], want, (32 + e / 8) * E * want.abs(), "weights")
+        g = want * (dweights[rows].double() - (want * dweights[rows].double()).sum(1, keepdim=True))
+        full = torch.zeros(64, e, dtype=torch.float64, device="cuda").scatter_(1, want_ids.long(), g)
+        bounded(back[rows], full, 320 * E * 2 + STEP[torch.bfloat16] * full.abs(), "dlogits")
+    assert ids[1000000].tolist() == [0, 1, 2, 3]
