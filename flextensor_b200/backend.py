@@ -878,7 +878,8 @@ def expert_linear_backward(x, weight, plan, dy, dx=None, dweight=None, dbias=Non
     """Gradients of ``expert_linear`` from dy[rows,N]: dx[rows,K] by place, dweight (shape of weight), dbias (shape of
     bias), zeros for an expert without rows; each may be None, not all.  With ``gather`` the gradient of x is the sum of
     its places: ``expert_combine(dx, plan, out)``.  Places past the last row are neither read nor written.
-    ``workspace``: at least ``expert_linear_backward_workspace_bytes(plan, N, K, gated)`` bytes."""
+    ``workspace``: at least ``expert_linear_backward_workspace_bytes(plan, N, K, gated)`` bytes, not shared with a call that
+    may run at the same time."""
     dtype = _element(x, "x")
     act = _one_of(activation, ACTIVATIONS, "activation")
     _plan_of(plan)

@@ -9,7 +9,8 @@
 //               row past the end of its expert is asked for outside the tensor, which fills it with zeros
 //   warp 1, 2   issuers of tcgen05.mma, one per A sub-tile.  The whole warp runs the loop and one elected lane issues:
 //               addresses and descriptors then stay in uniform registers.  Run by a single lane, a stage of four MMAs
-//               took about 900 cycles whatever its tile, now 500 in a pair and 420 alone (256 x 4096 x 4096: 31.4 -> 20.9 us)
+//               took about 900 cycles whatever its tile, now 500 in a pair and 420 alone (256 x 4096 x 4096: 31.4 -> 20.9 us
+//               when it was changed; 23.3 as it stands)
 //   warp 3      second loader where rows are fetched by number (a gather4 costs its loader about 50 ns)
 //   warps 4..   epilogue: tcgen05.ld -> bias, activation, gate, residual -> stores
 //
@@ -23,17 +24,18 @@
 // Waits are bounded as in ftb_umma_kernel.cuh: a role that gives up sets a status bit and the CTA leaves through its
 // normal teardown.
 //
-// What bounds it, measured on a B200 (bf16, device time in a CUDA graph of calls on rotating operands):
-//   4096 x 4096 x 4096            95 us   1447 TFLOP/s, 0.89 of the measured matrix rate; rows through the SM's port (256 a
-//                                         stage for 512 cycles of math) and the power cap
-//   8192 x (2 x 8192) x 4096 gated 812 us 1354 TFLOP/s, 0.97 of the sustained rate: the power cap
-//   1 x 4096 x 4096               9.3 us  3.6 TB/s: 5.1 us of reading W, then launch, first copies and the exchange of the
-//                                         partial sums; eight CTAs per tile (four: 9.4, two: 13.5, one: 19.7)
-//   48 x (2 x 8192) x 2048 gated  16.6 us 4.0 TB/s: 10.4 us of reading W
-//   1237 x 2048 x 1000            10.9 us, with GELU, bias, residual and preact 15.8: one wave of tiles whose epilogue
-//                                         nothing covers; 2051 columns, stored in 2-byte accesses: 16.4
-//   16384 places of 32 experts x 2048 x 2048  122 us  1.06 PFLOP/s of useful work: a quarter of the tiles' rows are the ends
-//                                         of groups; the same rows gathered by number 167 us (12 cycles a row)
+// What bounds it, measured on a B200 (bf16, device time in a CUDA graph of calls on rotating operands larger than L2, after
+// 0.4 s of the same load, so under the power cap where it applies; in brackets the first milliseconds):
+//   4096 x 4096 x 4096            114 us  1.20 PFLOP/s at 1485 MHz, 0.86 of the sustained matrix rate (97 us, 1.41, 0.87 of
+//                                         the burst rate); rows through the SM's port (256 a stage for 512 cycles of math)
+//   8192 x (2 x 8192) x 4096 gated 862 us 1.28 PFLOP/s at 1425 MHz, 0.91 of the sustained rate (809 us): the power cap
+//   1 x 4096 x 4096               9.7 us  3.4 TB/s: 5.1 us of reading W, then launch, first copies and the exchange of the
+//                                         partial sums; four CTAs per tile (eight: 11.7, two: 13.6, one: 21.4)
+//   48 x (2 x 8192) x 2048 gated  16.9 us 4.0 TB/s: 10.4 us of reading W
+//   1237 x 2048 x 1000            10.6 us, with GELU, bias, residual and preact 15.6: one wave of tiles whose epilogue
+//                                         nothing covers; 2051 columns, stored in 2-byte accesses: 16.2
+//   15360 places of 32 experts x 2048 x 2048  156 us  0.82 PFLOP/s of useful work (132 us, 0.98): a quarter of the tiles' rows
+//                                         are the ends of groups; the same rows gathered by number 186 us (12 cycles a row)
 #include "ftb_linear.h"
 #include "ftb_ptx.cuh"
 #include "ftb_tmap.h"
@@ -163,7 +165,7 @@ __device__ __forceinline__ void act_values(float (&v)[NC], int act) {
 // the accumulator lies, a feature per lane.  Where every row of the results starts on 16 bytes (`vec`) a warp then turns
 // its 16 x 32 values round through 2.25 KB of shared memory and a lane loads and stores eight features of a token at a
 // time.  Rows of other pitches keep 2-byte accesses, 64 contiguous bytes per warp, without predicates where all columns
-// are tokens (GELU with bias, residual and preact, 1237 x 2048 x 1000: 15.8 us; 2051 columns: 16.4, with predicates 21.2).
+// are tokens (GELU with bias, residual and preact, 1237 x 2048 x 1000: 15.6 us; 2051 columns: 16.2, with predicates 21.2).
 constexpr int kCols = 16;          // columns a thread holds at a time
 constexpr int kTurnPitch = 36;     // floats between two tokens: a lane's 16-byte reads meet no bank twice
 constexpr int kTurnFloats = kCols * kTurnPitch;
@@ -809,7 +811,7 @@ struct LinPick {
   bool pair;
   int form, bn, split;
   bool deep;  // single CTAs with an SM's shared memory each: no more of them than SMs, and clusters of at most four
-              // (eight such CTAs find room in a GPC twice at best: 22 us for 8 x 2048 x 8192, 10 with two CTAs an SM)
+              // (eight such CTAs find room in a GPC twice at best: 22 us for 8 x 2048 x 8192, 10.6 with two CTAs an SM)
 };
 
 static size_t stage_size(const LinPick& c) {
@@ -846,8 +848,9 @@ static int64_t most_tiles(const LinArgs& q, const LinPick& c) {
 //   and for preact, half as many again in 2-byte accesses; it runs under the next tile's main loop where a second
 //   accumulator exists;
 //   a split reduction costs two cluster barriers and the exchange of its columns.
-// Estimates against measurements: 1 x 4096 x 4096 split 8 / 4 / 2: 9.0 / 9.4 / 13.5 us measured; 256 x 4096 x 4096 pairs of
-// 64 / 256 tokens 20.8 / 25.5; 1237 x 2048 x 1000 pairs of 160 / 256 tokens 15.7 / 20.1, single CTAs of 96 tokens 21.4.
+// What it has to tell apart, measured: 1 x 4096 x 4096 split 8 / 4 / 2: 11.7 / 9.7 / 13.6 us; 256 x 4096 x 4096 pairs of
+// 64 / 128 / 256 tokens 23.3 / 23.9 / 25.3; 1237 x 2048 x 1000 with a rich epilogue, pairs of 160 / 256 tokens 15.6 / 20.1,
+// single CTAs of 128 tokens 24.4.
 static double variant_cycles(const LinArgs& q, LinPick c, int sms) {
   c.deep = !c.pair && c.split <= 4 && most_tiles(q, c) * c.split <= sms;
   const double blocks = q.mode == LIN_REDUCE ? static_cast<double>(q.rows) / q.groups / kKBlock + 0.5

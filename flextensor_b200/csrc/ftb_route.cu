@@ -11,11 +11,14 @@
 // sorting network puts them in descending order once; every one of the top_k rounds then is a maximum over 32 heads and
 // a shift in the winning lane.  The bits given to the place widen the distance that counts as near.
 //
-// Measured (fp32 logits, device time): 16384 x 256 in 8 groups of which 4 stay, sigmoid with bias, top 8: 23.4 us, where
+// Measured (fp32 logits, device time): 16384 x 256 in 8 groups of which 4 stay, sigmoid with bias, top 8: 23.8 us, where
 // reading the rows takes 2.7: bound by the latency of the choice (a reduction, a vote and a shift per round) at 40 warps an
-// SM; without bias and groups 13.9 us; 16384 x 64 softmax, top 6: 11.6 us; 16 x 64: 3.3 us, one launch.  A row that needs
-// 64 bits adds 4.6 us of latency to the launch that meets it (3 in 1000 rows of the first case do, so it is the launch's
-// tail, not its sum).
+// SM; without bias and groups 14.4 us; 16384 x 64 softmax, top 6: 11.7 us; 16 x 64: 2.9 us, one launch.
+// A row that needs 64 bits adds 4.6 us of latency to the launch that meets it.  3 in 1000 rows of the first case do, so it is
+// the launch's tail, not its sum.  More do where scores come from 16-bit logits that tie, in groups and without a bias: 32 %
+// of normal bf16 rows of that size (fp16 5 %), 42.6 us (26.8) instead of 22.2; 13 % of 64 experts, 17.5 instead of 13.7.  All
+// do where a large finite bias masks experts, since the bound grows with it (-1e4 or -1e9: 64 us, 27 for 64 experts; a mask
+// of -inf costs nothing), and where neither a score nor the bias reaches 2e-3 (the same times).
 #include "ftb_lm.cuh"
 
 namespace ftb {

@@ -267,8 +267,10 @@ int ftb_dwconv2d_nchw_f32_multi(const float* in, const float* weight, const floa
  * No counterpart in the reference, whose contractions end with the plain product (flextensor/nn/ops.py:1074-1158).
  * Conventions beyond the ones above: tensors are contiguous; `tokens` or `rows` of 0 is a call with nothing to
  * multiply (gradients of weights and biases are then written as zeros); matrix elements are 16 bits wide, every sum is
- * carried in fp32 and rounded once when it is stored.  Row pitches and bases that are multiples of 16 bytes (`k`, and
- * for gradients nothing else, a multiple of 8) run on tcgen05; other sizes run on a CUDA-core kernel of the library. */
+ * carried in fp32 and rounded once when it is stored - between two calls (the experts' rows before their weighted sum,
+ * dx by place before the sum over a token's places) results are 16-bit tensors, too.  Row pitches and bases that are
+ * multiples of 16 bytes (`k`, and for gradients nothing else, a multiple of 8) run on tcgen05; other sizes run on a
+ * CUDA-core kernel of the library (2048 x 2048 x 1001: 563 us, against 13 with k = 1000). */
 enum ftb_dtype { FTB_F32 = 0, FTB_BF16 = 1, FTB_F16 = 2 };
 enum ftb_activation { FTB_ACT_NONE = 0, FTB_ACT_RELU = 1, FTB_ACT_GELU = 2 /* erf */, FTB_ACT_GELU_TANH = 3, FTB_ACT_SILU = 4 };
 enum ftb_scoring { FTB_SCORE_SOFTMAX = 0, FTB_SCORE_SIGMOID = 1 };
