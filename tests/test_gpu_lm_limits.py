@@ -367,3 +367,18 @@ def test_logits_past_32_bits(B):
         full = torch.zeros(64, e, dtype=torch.float64, device="cuda").scatter_(1, want_ids.long(), g)
         bounded(back[rows], full, 320 * E * 2 + STEP[torch.bfloat16] * full.abs(), "dlogits")
     assert ids[1000000].tolist() == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_slopes_at_zero(B, status, act, gated):
+    """z of 0 and -0: relu's slope is 0 there, as the entry says, GELU's and SiLU's one half."""
+    n, k = 16, 64
+    z = torch.tensor([0.0, -0.0] * 8, dtype=torch.bfloat16)[None]
+    zz = torch.cat([z, torch.full_like(z, 3.0)], dim=1).cuda() if gated else z.cuda()
+    dy, db = torch.full((1, n), 2.0, device="cuda", dtype=torch.bfloat16), torch.empty(zz.shape[1], device="cuda", dtype=torch.bfloat16)
+    ws = torch.empty(B.linear_backward_workspace_bytes(1, n, k, gated), dtype=torch.uint8, device="cuda")
+    w = rand(2, zz.shape[1], k)
+    B.linear_backward(rand(1, 1, k), w, dy, dbias=db, preact=zz, activation=act, gated=gated, workspace=ws, status=status)
+    slope = {"none": 1.0, "relu": 0.0}.get(act, 0.5)
+    assert (db[:n] == 2 * slope * (3 if gated else 1)).all() and not db[n:].any()
